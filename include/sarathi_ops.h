@@ -356,6 +356,96 @@ int sarathi_rotary_embedding_append_paged_kv(
     void* stream);
 
 /*
+ * New entry: the index vectors of a hybrid batch from the requests' lengths, on the GPU; stands for
+ * the host loops and copies of FlashinferAttentionWrapper.begin_forward
+ * (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:84-229).
+ * query_lens / seq_lens [num_seqs]: new tokens, and tokens in all after the append (negative counts
+ * as 0).  block_tables [num_seqs, max_pages_per_seq], rows table_stride entries apart: the pages of
+ * each sequence in order, of which the first p = min(ceil(seq_len / page_size), max_pages_per_seq)
+ * are in use.  Written:
+ *   qo_indptr, kv_indptr [num_seqs + 1]  exclusive prefix sums of the new tokens and of p, held at
+ *                                        num_tokens and num_kv_pages where the sums pass them
+ *   kv_indices [num_kv_pages]            the used pages of all sequences in a row, -1 behind them
+ *   kv_last_page_len [num_seqs]          entries of the last used page (0 without a page)
+ *   batch_indices, positions, slot_mapping [num_tokens] and rope_positions (int64) [num_tokens]:
+ *     sequence, index in the sequence, page * page_size + entry of every new token, and the index
+ *     again as sarathi_rotary_embedding takes it.  Tokens behind the last sequence get -1, -1, -1,
+ *     0; a token whose index is negative (query_len > seq_len) or past its table row gets position
+ *     and slot -1, one whose page number is negative slot -1.  The append entries skip both.
+ * num_tokens and num_kv_pages are the lengths of those vectors, which the host knows; a larger
+ * value leaves room for the batches of a captured graph.  page * page_size must stay below 2^31.
+ */
+int sarathi_build_paged_kv_metadata(const int32_t* query_lens, const int32_t* seq_lens,
+                                    const int32_t* block_tables, int32_t* qo_indptr,
+                                    int32_t* kv_indptr, int32_t* kv_indices,
+                                    int32_t* kv_last_page_len, int32_t* batch_indices,
+                                    int32_t* positions, int32_t* slot_mapping,
+                                    int64_t* rope_positions, int64_t num_seqs,
+                                    int64_t max_pages_per_seq, int64_t table_stride, int page_size,
+                                    int64_t num_tokens, int64_t num_kv_pages, void* stream);
+
+/*
+ * New entry: attention of a batch's new tokens over the paged cache, chunks of prompts and single
+ * decode tokens in one call; stands for the flashinfer wrappers that the reference plans and runs
+ * (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:169-209, 275-304).
+ * query / out [num_tokens, num_heads, head_size], tokens query_stride / out_stride elements apart;
+ * the tokens of request r are [qo_indptr[r], qo_indptr[r + 1]), its keys and values the first
+ * (pages - 1) * page_size + kv_last_page_len[r] entries of the pages
+ * kv_indices[kv_indptr[r] .. kv_indptr[r + 1]); the cache geometry is that of
+ * sarathi_append_paged_kv_cache.  Query head h uses key head h / (num_heads / num_kv_heads).
+ * With n new tokens and s keys, new token j has index x = s - n + j and sees keys i <= x (causal),
+ * of these i >= x - window_left (window_left >= 0), scaled by sm_scale:
+ *   lse = log sum_i exp(sm_scale <q, k_i>),   out = sum_i exp(sm_scale <q, k_i> - lse) v_i.
+ * A token that sees no key gets out = 0, lse = -inf.  lse (float [num_tokens, num_heads], natural
+ * logarithm) may be NULL.  Rows of out and lse outside [qo_indptr[0], qo_indptr[num_seqs]) are left
+ * as they were.  dtype bfloat16 / float16, head_size up to 256 (multiples of 8 with 16-byte aligned
+ * rows take the matrix cores, anything else a plain kernel).  Sums, maxima and the output are held
+ * in 32 bits; the probabilities are rounded to dtype for their product with the values.
+ *
+ * Lengths are read on the GPU, so a captured call follows what the index vectors hold at replay.
+ * Index vectors must not decrease; whatever they hold, nothing outside the tensors is touched, and
+ * a page number outside [0, num_pages) is not followed (the last page stands in for it).  Entries
+ * past a request's last key are not read; entries of the request itself that a mask hides from some
+ * of its tokens must be finite.
+ *
+ * max_query_len (0: unknown) is an upper bound of the new tokens of any request; it picks the
+ * kernel, and a wrong one costs time, not correctness.  workspace: scratch of
+ * sarathi_paged_attention_workspace_bytes() bytes, 16-byte aligned, for the states of contexts that
+ * are cut into parts to fill the GPU; contents irrelevant on entry and exit, not shared by calls
+ * that may overlap.  With NULL or less nothing is cut (slower for few long contexts).
+ */
+int64_t sarathi_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_seqs,
+                                                int64_t num_kv_indices, int num_heads,
+                                                int num_kv_heads, int head_size, int page_size,
+                                                int64_t max_query_len);
+int sarathi_paged_attention(const void* query, const void* k_cache, const void* v_cache, void* out,
+                            float* lse, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                            const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                            int64_t num_tokens, int64_t num_seqs, int64_t num_kv_indices,
+                            int64_t num_pages, int num_heads, int num_kv_heads, int head_size,
+                            int page_size, int64_t query_stride, int64_t out_stride,
+                            int64_t page_stride, int64_t entry_stride, float sm_scale, int causal,
+                            int64_t window_left, int64_t max_query_len, void* workspace,
+                            int64_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * New entry: joins attention states computed over disjoint parts of a context (e.g. a prefix that
+ * requests share and each request's own suffix).  For every token and head, with the states'
+ * outputs v (v_state_stride apart, tokens v_token_stride apart, [num_heads, head_size] contiguous)
+ * and natural-log lse (lse_state_stride, lse_token_stride, heads contiguous):
+ *   out_lse = log sum_s exp(lse_s),   out = sum_s exp(lse_s - out_lse) v_s,
+ * sums in 32 bits, one rounding.  A state with lse = -inf is left out whatever its v holds; with no
+ * other state out = 0 and out_lse = -inf.  out_lse may be NULL.  dtype (of v and out): float32,
+ * float16, bfloat16.  out and out_lse must not overlap v and lse.
+ */
+int sarathi_merge_attention_states(const void* v, const float* lse, void* out, float* out_lse,
+                                   int64_t num_states, int64_t num_tokens, int num_heads,
+                                   int head_size, int64_t v_state_stride, int64_t v_token_stride,
+                                   int64_t lse_state_stride, int64_t lse_token_stride,
+                                   int64_t out_token_stride, int64_t out_lse_token_stride,
+                                   int dtype, void* stream);
+
+/*
  * No counterpart in the reference: spreads every expert's slots evenly over the blocks that
  * sarathi_moe_align_block_size gave it (fused_moe.py:151-204 fills them greedily, so an expert's
  * last block is often nearly empty; such blocks cost the grouped GEMM far more than their share

@@ -2,6 +2,8 @@
 // launch-status query.  Entry points never synchronise, allocate or throw.
 #pragma once
 
+#include <atomic>
+
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -18,6 +20,21 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 // per-thread and clears the sticky value).
 static inline int launch_status() {
   return hipGetLastError() == hipSuccess ? SARATHI_OK : SARATHI_ERR_LAUNCH;
+}
+
+// Lets kernel K take `bytes` of dynamic shared memory, which may be more than the default limit per
+// workgroup: asked for once per kernel and device (racing first calls both ask: harmless).
+template <auto K> static inline bool allow_lds(int bytes) {
+  static std::atomic<bool> raised[64] = {};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+  if (!raised[dev].load(std::memory_order_acquire)) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(K),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return false;
+    raised[dev].store(true, std::memory_order_release);
+  }
+  return true;
 }
 
 // Compute units of the current device (looked up once; 256 when the query fails).

@@ -398,6 +398,158 @@ void rotary_embedding_append_paged_kv(torch::Tensor& positions, torch::Tensor& q
            op);
 }
 
+// the index vectors of a batch from its lengths; see include/sarathi_ops.h for what they hold
+void build_paged_kv_metadata(torch::Tensor& query_lens, torch::Tensor& seq_lens,
+                             torch::Tensor& block_tables, torch::Tensor& qo_indptr,
+                             torch::Tensor& kv_indptr, torch::Tensor& kv_indices,
+                             torch::Tensor& kv_last_page_len, torch::Tensor& batch_indices,
+                             torch::Tensor& positions, torch::Tensor& slot_mapping,
+                             torch::Tensor& rope_positions, int64_t page_size) {
+  const char* op = "build_paged_kv_metadata";
+  check_i32(query_lens, query_lens, op, "query_lens");
+  check_i32(seq_lens, query_lens, op, "seq_lens");
+  check_gpu(block_tables, query_lens, op, "block_tables");
+  check_i32(qo_indptr, query_lens, op, "qo_indptr");
+  check_i32(kv_indptr, query_lens, op, "kv_indptr");
+  check_i32(kv_indices, query_lens, op, "kv_indices");
+  check_i32(kv_last_page_len, query_lens, op, "kv_last_page_len");
+  check_i32(batch_indices, query_lens, op, "batch_indices");
+  check_i32(positions, query_lens, op, "positions");
+  check_i32(slot_mapping, query_lens, op, "slot_mapping");
+  check_gpu(rope_positions, query_lens, op, "rope_positions");
+  const int64_t n = query_lens.numel(), t = positions.numel();
+  TORCH_CHECK(page_size > 0 && page_size <= INT32_MAX, op, ": page_size must be positive");
+  TORCH_CHECK(seq_lens.numel() == n && kv_last_page_len.numel() == n && qo_indptr.numel() == n + 1 &&
+                  kv_indptr.numel() == n + 1,
+              op, ": expected query_lens, seq_lens and kv_last_page_len [n], qo_indptr and kv_indptr [n+1]");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == n &&
+                  block_tables.scalar_type() == at::ScalarType::Int &&
+                  (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
+              op, ": block_tables must be int32 [num_seqs, max_pages] with contiguous rows");
+  TORCH_CHECK(n <= 1 || block_tables.stride(0) >= block_tables.size(1), op,
+              ": the rows of block_tables must not overlap");
+  TORCH_CHECK(batch_indices.numel() == t && slot_mapping.numel() == t && rope_positions.numel() == t &&
+                  rope_positions.scalar_type() == at::ScalarType::Long && rope_positions.is_contiguous(),
+              op, ": the per-token vectors must hold num_tokens entries, rope_positions int64");
+  LaunchScope scope(query_lens);
+  raise_on(sarathi_build_paged_kv_metadata(
+               query_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+               block_tables.data_ptr<int32_t>(), qo_indptr.data_ptr<int32_t>(),
+               kv_indptr.data_ptr<int32_t>(), kv_indices.data_ptr<int32_t>(),
+               kv_last_page_len.data_ptr<int32_t>(), batch_indices.data_ptr<int32_t>(),
+               positions.data_ptr<int32_t>(), slot_mapping.data_ptr<int32_t>(),
+               rope_positions.data_ptr<int64_t>(), n, block_tables.size(1),
+               n > 1 ? block_tables.stride(0) : block_tables.size(1), (int)page_size, t,
+               kv_indices.numel(), scope.stream),
+           op);
+}
+
+// attention of the batch's new tokens over the paged cache.  The scratch for cut contexts comes from
+// torch's caching allocator on the launch stream, so calls never share it.
+void paged_attention(torch::Tensor& query, torch::Tensor& k_cache, torch::Tensor& v_cache,
+                     torch::Tensor& qo_indptr, torch::Tensor& kv_indptr, torch::Tensor& kv_indices,
+                     torch::Tensor& kv_last_page_len, torch::Tensor& out,
+                     c10::optional<torch::Tensor> lse, double sm_scale, bool causal,
+                     int64_t window_left, int64_t max_query_len) {
+  const char* op = "paged_attention";
+  check_gpu(query, query, op, "query");
+  check_gpu(k_cache, query, op, "k_cache");
+  check_gpu(v_cache, query, op, "v_cache");
+  check_gpu(out, query, op, "out");
+  check_i32(qo_indptr, query, op, "qo_indptr");
+  check_i32(kv_indptr, query, op, "kv_indptr");
+  check_i32(kv_indices, query, op, "kv_indices");
+  check_i32(kv_last_page_len, query, op, "kv_last_page_len");
+  TORCH_CHECK(query.scalar_type() == at::ScalarType::Half ||
+                  query.scalar_type() == at::ScalarType::BFloat16,
+              op, ": only bfloat16 and float16 are supported, got ", query.scalar_type());
+  TORCH_CHECK(k_cache.scalar_type() == query.scalar_type() &&
+                  v_cache.scalar_type() == query.scalar_type() &&
+                  out.scalar_type() == query.scalar_type(),
+              op, ": query, out and the cache must share a dtype");
+  const PagedGeom g = paged_geom(k_cache, v_cache, op);
+  TORCH_CHECK(g.heads > 0 && g.head_size > 0 && g.page_size > 0, op, ": the cache has no entries");
+  TORCH_CHECK(g.head_size <= 256, op, ": head_size must be at most 256, got ", g.head_size);
+  TORCH_CHECK(query.dim() == 2 || query.dim() == 3, op,
+              ": query must be [tokens, heads, head_size] or [tokens, heads * head_size]");
+  const int64_t width = query.dim() == 2 ? query.size(1) : query.size(1) * query.size(2);
+  TORCH_CHECK(width > 0 && width % (g.heads * g.head_size) == 0, op,
+              ": the query heads must be a multiple of the cache's ", g.heads, " heads of ",
+              g.head_size);
+  const int64_t qs = token_rows(query, width, g.head_size, op, "query");
+  TORCH_CHECK(out.sizes() == query.sizes(), op, ": out and query shapes differ");
+  const int64_t os = token_rows(out, width, g.head_size, op, "out");
+  const int64_t tokens = query.size(0), heads = width / g.head_size;
+  const int64_t seqs = kv_last_page_len.numel();
+  TORCH_CHECK(qo_indptr.numel() == seqs + 1 && kv_indptr.numel() == seqs + 1, op,
+              ": expected qo_indptr and kv_indptr [n+1], kv_last_page_len [n]");
+  TORCH_CHECK(tokens <= 1 || (qs >= width && os >= width), op, ": rows must not overlap");
+  float* lse_ptr = nullptr;
+  if (lse.has_value()) {
+    check_gpu(*lse, query, op, "lse");
+    TORCH_CHECK(lse->scalar_type() == at::ScalarType::Float && lse->is_contiguous() &&
+                    lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == heads,
+                op, ": lse must be contiguous float32 [tokens, heads]");
+    lse_ptr = lse->data_ptr<float>();
+  }
+  TORCH_CHECK(max_query_len >= 0, op, ": max_query_len must not be negative");
+  TORCH_CHECK(heads <= 65535 && g.page_size <= INT32_MAX, op, ": too many heads or entries");
+  LaunchScope scope(query);
+  const int64_t ws = sarathi_paged_attention_workspace_bytes(
+      tokens, seqs, kv_indices.numel(), (int)heads, (int)g.heads, (int)g.head_size,
+      (int)g.page_size, max_query_len);
+  torch::Tensor workspace;
+  if (ws > 0) workspace = torch::empty({ws}, query.options().dtype(torch::kUInt8));
+  raise_on(sarathi_paged_attention(
+               query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse_ptr,
+               qo_indptr.data_ptr<int32_t>(), kv_indptr.data_ptr<int32_t>(),
+               kv_indices.data_ptr<int32_t>(), kv_last_page_len.data_ptr<int32_t>(), tokens, seqs,
+               kv_indices.numel(), k_cache.size(0), (int)heads, (int)g.heads, (int)g.head_size,
+               (int)g.page_size, tokens > 1 ? qs : width, tokens > 1 ? os : width, g.page_stride,
+               g.entry_stride, (float)sm_scale, causal ? 1 : 0, window_left, max_query_len,
+               ws > 0 ? workspace.data_ptr() : nullptr, ws, dtype_code(query, op), scope.stream),
+           op);
+}
+
+// joins states [S, T, H, D] with their lse [S, T, H]; the state and token dimensions may have any
+// strides
+void merge_attention_states(torch::Tensor& v, torch::Tensor& lse, torch::Tensor& out,
+                            c10::optional<torch::Tensor> out_lse) {
+  const char* op = "merge_attention_states";
+  check_gpu(v, v, op, "v");
+  check_gpu(lse, v, op, "lse");
+  check_gpu(out, v, op, "out");
+  const int code = dtype_code(v, op);
+  TORCH_CHECK(v.dim() == 4 && lse.dim() == 3 && lse.size(0) == v.size(0) && lse.size(1) == v.size(1) &&
+                  lse.size(2) == v.size(2),
+              op, ": expected v [states, tokens, heads, head_size] and lse [states, tokens, heads]");
+  const int64_t S = v.size(0), T = v.size(1), H = v.size(2), D = v.size(3);
+  TORCH_CHECK(S >= 1 && H > 0 && D > 0, op, ": there must be a state, a head and an element");
+  TORCH_CHECK((v.stride(3) == 1 || D == 1) && (v.stride(2) == D || H == 1), op,
+              ": the [heads, head_size] part of v must be contiguous");
+  TORCH_CHECK(lse.scalar_type() == at::ScalarType::Float && (lse.stride(2) == 1 || H == 1), op,
+              ": lse must be float32 with contiguous heads");
+  TORCH_CHECK(out.dim() == 3 && out.size(0) == T && out.size(1) == H && out.size(2) == D &&
+                  out.is_contiguous() && out.scalar_type() == v.scalar_type(),
+              op, ": out must be contiguous [tokens, heads, head_size] of v's dtype");
+  TORCH_CHECK(T <= 1 || (v.stride(1) >= H * D && lse.stride(1) >= H), op, ": rows must not overlap");
+  float* out_lse_ptr = nullptr;
+  if (out_lse.has_value()) {
+    check_gpu(*out_lse, v, op, "out_lse");
+    TORCH_CHECK(out_lse->scalar_type() == at::ScalarType::Float && out_lse->is_contiguous() &&
+                    out_lse->dim() == 2 && out_lse->size(0) == T && out_lse->size(1) == H,
+                op, ": out_lse must be contiguous float32 [tokens, heads]");
+    out_lse_ptr = out_lse->data_ptr<float>();
+  }
+  TORCH_CHECK(H <= INT32_MAX && D <= INT32_MAX, op, ": too many heads or elements");
+  LaunchScope scope(v);
+  raise_on(sarathi_merge_attention_states(
+               v.data_ptr(), lse.data_ptr<float>(), out.data_ptr(), out_lse_ptr, S, T, (int)H, (int)D,
+               v.stride(0), T > 1 ? v.stride(1) : H * D, lse.stride(0), T > 1 ? lse.stride(1) : H,
+               H * D, H, code, scope.stream),
+           op);
+}
+
 // ---- moe_ops -----------------------------------------------------------------
 
 void topk_softmax_impl(torch::Tensor& topk_weights, torch::Tensor& topk_indices,
@@ -831,6 +983,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("k_cache"), pybind11::arg("v_cache"), pybind11::arg("kv_indices"),
         pybind11::arg("kv_indptr"), pybind11::arg("num_append_tokens"),
         pybind11::arg("write_key"), pybind11::arg("slot_mapping") = pybind11::none());
+  m.def("build_paged_kv_metadata", &build_paged_kv_metadata,
+        "index vectors of a hybrid batch from its lengths and page tables",
+        pybind11::arg("query_lens"), pybind11::arg("seq_lens"), pybind11::arg("block_tables"),
+        pybind11::arg("qo_indptr"), pybind11::arg("kv_indptr"), pybind11::arg("kv_indices"),
+        pybind11::arg("kv_last_page_len"), pybind11::arg("batch_indices"),
+        pybind11::arg("positions"), pybind11::arg("slot_mapping"), pybind11::arg("rope_positions"),
+        pybind11::arg("page_size"));
+  m.def("paged_attention", &paged_attention,
+        "attention of a hybrid batch's new tokens over a paged (NHD) KV cache",
+        pybind11::arg("query"), pybind11::arg("k_cache"), pybind11::arg("v_cache"),
+        pybind11::arg("qo_indptr"), pybind11::arg("kv_indptr"), pybind11::arg("kv_indices"),
+        pybind11::arg("kv_last_page_len"), pybind11::arg("out"), pybind11::arg("lse"),
+        pybind11::arg("sm_scale"), pybind11::arg("causal") = true,
+        pybind11::arg("window_left") = -1, pybind11::arg("max_query_len") = 0);
+  m.def("merge_attention_states", &merge_attention_states,
+        "join attention states computed over disjoint parts of a context", pybind11::arg("v"),
+        pybind11::arg("lse"), pybind11::arg("out"), pybind11::arg("out_lse") = pybind11::none());
   // moe_ops
   m.def("topk_softmax", &topk_softmax, "softmax over experts + top-k (raw probabilities)");
   m.def("topk_softmax_renorm", &topk_softmax_renorm,

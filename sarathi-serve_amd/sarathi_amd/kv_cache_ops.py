@@ -1,12 +1,13 @@
 """Paged KV-cache append ops with the signatures of the flashinfer functions the reference's
 attention wrapper calls (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:213-226
-and :262-273; flashinfer-python==0.4.1), plus the rotary-embedding + append fusion.
+and :262-273; flashinfer-python==0.4.1), plus the rotary-embedding + append fusion, the index
+vectors of a batch built on the GPU, attention over the cache and the join of attention states.
 
 The cache is flashinfer's NHD layout: one tensor ``[num_pages, 2, page_size, num_kv_heads,
 head_size]`` (K plane, V plane) or a ``(k_cache, v_cache)`` pair of
 ``[num_pages, page_size, num_kv_heads, head_size]`` tensors.
 """
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -89,5 +90,93 @@ def rotary_embedding_append_paged_kv(positions: torch.Tensor, query: torch.Tenso
                                         kv_indices, kv_indptr, n, write_key, slot_mapping)
 
 
+class PagedKvMetadata(NamedTuple):
+    """What ``build_paged_kv_metadata`` returns; the names of the append's and the attention's
+    arguments.  int32 but for ``rope_positions``."""
+    qo_indptr: torch.Tensor         # [num_seqs + 1] start of each sequence's new tokens
+    kv_indptr: torch.Tensor         # [num_seqs + 1] start of each sequence's pages
+    kv_indices: torch.Tensor        # [num_kv_pages] used pages of all sequences in a row, then -1
+    kv_last_page_len: torch.Tensor  # [num_seqs]
+    batch_indices: torch.Tensor     # [num_tokens] sequence of every new token
+    positions: torch.Tensor         # [num_tokens] its index in the sequence
+    slot_mapping: torch.Tensor      # [num_tokens] page * page_size + entry
+    rope_positions: torch.Tensor    # [num_tokens] int64, for the rotary embedding
+
+
+def build_paged_kv_metadata(query_lens: torch.Tensor, seq_lens: torch.Tensor,
+                            block_tables: torch.Tensor, page_size: int, num_tokens: int,
+                            num_kv_pages: Optional[int] = None) -> PagedKvMetadata:
+    """The index vectors of a batch from lengths that live on the GPU, without a copy or a
+    synchronisation: the device-side counterpart of FlashinferAttentionWrapper.begin_forward's
+    bookkeeping (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:84-229).
+
+    ``query_lens`` / ``seq_lens`` int32 ``[num_seqs]``: new tokens, and tokens in all after the
+    append.  ``block_tables`` int32 ``[num_seqs, max_pages]``: each sequence's pages in order;
+    entries past ``ceil(seq_len / page_size)`` are not read.  ``num_tokens`` and ``num_kv_pages``
+    (default: the size of ``block_tables``) are the lengths of the per-token vectors and of
+    ``kv_indices``; room beyond the batch, as a captured graph needs, is filled with -1
+    (``rope_positions``: 0), and the append ops skip negative slots and positions."""
+    if num_kv_pages is None:
+        num_kv_pages = block_tables.numel()
+    if num_tokens < 0 or num_kv_pages < 0:
+        raise ValueError("num_tokens and num_kv_pages must not be negative")
+    if page_size <= 0:
+        raise ValueError("page_size must be positive")
+    seqs = query_lens.numel()
+    # one allocation for the seven int32 vectors
+    sizes = [seqs + 1, seqs + 1, num_kv_pages, seqs, num_tokens, num_tokens, num_tokens]
+    flat = torch.empty((sum(sizes),), dtype=torch.int32, device=query_lens.device)
+    meta = PagedKvMetadata(*flat.split(sizes),
+                           torch.empty((num_tokens,), dtype=torch.int64, device=query_lens.device))
+    _C.build_paged_kv_metadata(query_lens, seq_lens, block_tables, *meta, page_size)
+    return meta
+
+
+def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: torch.Tensor,
+                    kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                    kv_last_page_len: torch.Tensor, sm_scale: Optional[float] = None,
+                    causal: bool = True, window_left: int = -1,
+                    max_query_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                    return_lse: bool = False, kv_layout: str = "NHD"):
+    """Attention of a batch's new tokens over their sequences in the cache, prompt chunks and single
+    decode tokens in one call (the two wrappers that the reference plans and runs at
+    sarathi/model_executor/attention/flashinfer_attention_wrapper.py:169-209 and :275-304).
+
+    ``query`` ``[num_tokens, num_heads, head_size]`` (or 2-D rows, possibly a view of a packed qkv
+    buffer), bfloat16 or float16; the tokens of request r are ``[qo_indptr[r], qo_indptr[r + 1])``
+    and are the last ones of its sequence, whose keys the four kv vectors describe as for the append.
+    With ``causal`` a token sees the keys up to its own, with ``window_left >= 0`` only that many
+    before it.  ``sm_scale`` defaults to ``head_size ** -0.5``.  ``max_query_len``, where the caller
+    knows an upper bound of the requests' new tokens, picks the kernel (1: a pure decode batch).
+
+    Returns ``out`` (shaped like ``query``), with ``return_lse`` also the natural-log sums
+    ``[num_tokens, num_heads]`` (float32) that ``merge_attention_states`` joins.  A token that sees no
+    key gets 0 and -inf; rows behind the last request are not written."""
+    k_cache, v_cache = _split_cache(paged_kv_cache, kv_layout)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    head_size = k_cache.shape[-1]
+    lse = None
+    if return_lse:
+        heads = query.shape[1] // head_size if query.dim() == 2 else query.shape[1]
+        lse = torch.empty((query.shape[0], heads), dtype=torch.float32, device=query.device)
+    _C.paged_attention(query, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
+                       out, lse, head_size ** -0.5 if sm_scale is None else sm_scale, causal,
+                       window_left, 0 if max_query_len is None else max_query_len)
+    return (out, lse) if return_lse else out
+
+
+def merge_attention_states(v: torch.Tensor, lse: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Joins ``paged_attention`` states over disjoint parts of a context, e.g. a prefix that requests
+    share and each request's own suffix: ``v`` ``[states, tokens, heads, head_size]``, ``lse``
+    ``[states, tokens, heads]`` (natural log, float32).  The state and token dimensions may have any
+    strides.  Returns the joined output and its lse; states with lse -inf are left out."""
+    out = torch.empty(v.shape[1:], dtype=v.dtype, device=v.device)
+    out_lse = torch.empty(lse.shape[1:], dtype=torch.float32, device=v.device)
+    _C.merge_attention_states(v, lse, out, out_lse)
+    return out, out_lse
+
+
 __all__ = ["get_seq_lens", "get_batch_indices_positions", "get_kv_slot_mapping", "append_paged_kv_cache",
-           "rotary_embedding_append_paged_kv"]
+           "rotary_embedding_append_paged_kv", "PagedKvMetadata", "build_paged_kv_metadata",
+           "paged_attention", "merge_attention_states"]
