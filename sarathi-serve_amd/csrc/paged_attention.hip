@@ -7,6 +7,7 @@
 // alignment, the kernel that joins the parts of a cut context, and the entry point that chooses.
 #include "launch.h"
 #include "paged_attn.h"
+#include "paged_attn_tiles.h"
 
 namespace sarathi_hip {
 
@@ -442,44 +443,92 @@ static int launch_join(const PagedAttnArgs& a, int rows_per_tile, hipStream_t st
 
 // ---- what a call launches ------------------------------------------------------------------------
 
-// Sizes that fix the launch, all known on the host.
-struct AttnPlan {
-  int row_tiles;       // few-rows kernel: 16 rows each
+// The requests of a batch fall into two classes by their rows (new tokens times query heads per key
+// head): few rows, and chunks, which take the tile kernel.  All sizes here are known on the host.
+struct AttnClass {
+  int rows;            // rows per tile, 0: the class is empty
+  int32_t min_rows, max_rows;
   int64_t tiles;       // at most so many tiles per key head
   int32_t target, min_part;
   int64_t items;       // at most so many items per key head
   int64_t map_bytes, ml_bytes, o_bytes;  // of the workspace
+  int64_t bytes() const { return map_bytes + ml_bytes + o_bytes; }
+};
+struct AttnPlan {
+  AttnClass few, tile;
 };
 static int64_t round256(int64_t v) { return (v + 255) & ~(int64_t)255; }
+
+// Aims at `items` work items per key head, of at least min_part keys each.
+static void plan_parts(AttnClass& c, int64_t items, int32_t min_part, int64_t seqs,
+                       int64_t capacity, int kv_heads, int head_size) {
+  const int64_t most = c.tiles * (capacity / min_part);  // no sequence is longer than all pages
+  c.min_part = min_part;
+  c.target = (int32_t)(items < most ? items : most);
+  c.items = c.tiles + c.target;
+  if (c.target <= 0) return;
+  c.map_bytes = round256((2 * seqs + 1) * 4);
+  c.ml_bytes = round256(c.items * kv_heads * c.rows * 8);
+  c.o_bytes = round256(c.items * kv_heads * c.rows * head_size * 4);
+}
 
 static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, int heads,
                                int kv_heads, int head_size, int page_size, int64_t max_query_len) {
   AttnPlan p{};
   const int group = heads / kv_heads;
-  int64_t longest = max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens;
-  const int64_t rows = longest * group;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  if (head_size > 128 && p.row_tiles > 2) p.row_tiles = 2;
-  const int per = 16 * p.row_tiles;
-  const int64_t all_rows = tokens * group;
-  p.tiles = all_rows / per + seqs;
-  if (p.tiles > all_rows) p.tiles = all_rows;
-  // Cutting: parts of at least 128 keys, two blocks per wave, and about as many items as two
-  // workgroups per compute unit need
-  p.min_part = 128;
-  const int64_t slots = 2 * compute_units();
-  int64_t target = slots / kv_heads > 0 ? slots / kv_heads : 1;
-  const int64_t capacity = indices * page_size;  // no sequence is longer
-  const int64_t most = p.tiles * (capacity / p.min_part);
-  if (target > most) target = most;
-  p.target = (int32_t)target;
-  p.items = p.tiles + p.target;
-  if (p.target > 0) {
-    p.map_bytes = round256((2 * seqs + 1) * 4);
-    p.ml_bytes = round256(p.items * kv_heads * per * 8);
-    p.o_bytes = round256(p.items * kv_heads * per * head_size * 4);
+  const int64_t longest = max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens;
+  const int64_t most_rows = longest * group, all_rows = tokens * group;
+  const int64_t capacity = indices * page_size;
+  const int units = compute_units();
+  const int few_limit = head_size > 128 ? 32 : 64;
+  AttnClass& f = p.few;
+  AttnClass& t = p.tile;
+  f.min_rows = 1;
+  if (most_rows <= few_limit || head_size > 128) {
+    // all requests in tiles of few rows (max_query_len may be wrong: any number of tiles each)
+    f.rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : few_limit;
+    f.max_rows = 0x7fffffff;
+    f.tiles = all_rows / f.rows + seqs;
+  } else {
+    // single tokens in one tile each, longer requests in large tiles
+    f.rows = group <= 16 ? 16 : group <= 32 ? 32 : few_limit;
+    f.max_rows = f.rows;
+    f.tiles = seqs;
+    t.min_rows = f.rows + 1;
+    t.max_rows = 0x7fffffff;
+    t.rows = all_rows / 256 * kv_heads >= units ? 256 : 128;
+    const int64_t chunks = seqs < all_rows / t.min_rows ? seqs : all_rows / t.min_rows;
+    t.tiles = all_rows / t.rows + chunks;
+    const int64_t fill = 2 * (int64_t)units / kv_heads;
+    plan_parts(t, t.tiles < fill ? (fill > 0 ? fill : 1) : 0, 512, seqs, capacity, kv_heads, head_size);
   }
+  if (f.tiles > all_rows) f.tiles = all_rows;
+  const int64_t fill = 2 * (int64_t)units / kv_heads;
+  plan_parts(f, fill > 0 ? fill : 1, 128, seqs, capacity, kv_heads, head_size);
   return p;
+}
+
+// Launches one class; `ws` is its part of the workspace or null.
+template <typename Launch>
+static int run_class(PagedAttnArgs a, const AttnClass& c, char* ws, int dtype, hipStream_t st,
+                     Launch launch) {
+  if (c.rows == 0) return SARATHI_OK;
+  a.min_rows = c.min_rows;
+  a.max_rows = c.max_rows;
+  const bool cut = c.target > 0 && ws;
+  if (cut) {
+    a.part_map = reinterpret_cast<int32_t*>(ws);
+    a.part_ml = reinterpret_cast<float*>(ws + c.map_bytes);
+    a.part_o = reinterpret_cast<float*>(ws + c.map_bytes + c.ml_bytes);
+    a.target = c.target;
+    a.min_part = c.min_part;
+  }
+  const int64_t groups = (cut ? c.items : c.tiles) * a.kv_heads;
+  if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
+  if (groups == 0) return SARATHI_OK;
+  const int rc = launch(a, groups);
+  if (rc != SARATHI_OK || !cut) return rc;
+  return dtype == kBF16 ? launch_join<kBF16>(a, c.rows, st) : launch_join<kF16>(a, c.rows, st);
 }
 
 }  // namespace sarathi_hip
@@ -507,7 +556,7 @@ extern "C" int64_t sarathi_paged_attention_workspace_bytes(int64_t num_tokens, i
     return 0;
   const AttnPlan p = plan_attention(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads,
                                     head_size, page_size, max_query_len);
-  return p.map_bytes + p.ml_bytes + p.o_bytes;
+  return p.few.bytes() + p.tile.bytes();
 }
 
 extern "C" int sarathi_paged_attention(
@@ -534,7 +583,7 @@ extern "C" int sarathi_paged_attention(
       num_pages >= 0x7fffffffLL)
     return SARATHI_ERR_UNSUPPORTED;
   if (num_tokens == 0 || num_seqs == 0) return SARATHI_OK;
-  AttnPlan p = plan_attention(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads,
+  const AttnPlan p = plan_attention(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads,
                               head_size, page_size, max_query_len);
   PagedAttnArgs a{};
   a.q = query;
@@ -566,8 +615,6 @@ extern "C" int sarathi_paged_attention(
   a.causal = causal != 0;
   a.window = window_left < 0 ? -1 : window_left < 0x3fffffff ? (int32_t)window_left : 0x3fffffff;
   a.scale_log2 = sm_scale * kLog2e;
-  a.min_rows = 1;
-  a.max_rows = 0x7fffffff;
   hipStream_t st = (hipStream_t)stream;
   const bool vec = head_size % 8 == 0 && aligned16(query) && aligned16(k_cache) &&
                    aligned16(v_cache) && aligned16(out) && query_stride % 8 == 0 &&
@@ -581,21 +628,16 @@ extern "C" int sarathi_paged_attention(
     return launch_status();
   }
   // a workspace that is missing or too small means no cutting, not an error
-  const bool cut = p.target > 0 && workspace && aligned16(workspace) &&
-                   workspace_bytes >= p.map_bytes + p.ml_bytes + p.o_bytes;
-  if (cut) {
-    char* w = reinterpret_cast<char*>(workspace);
-    a.part_map = reinterpret_cast<int32_t*>(w);
-    a.part_ml = reinterpret_cast<float*>(w + p.map_bytes);
-    a.part_o = reinterpret_cast<float*>(w + p.map_bytes + p.ml_bytes);
-    a.target = p.target;
-    a.min_part = p.min_part;
-  }
-  const int64_t groups = (cut ? p.items : p.tiles) * num_kv_heads;
-  if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
-  int rc = dtype == kBF16 ? launch_few_heads<kBF16>(a, p.row_tiles, groups, st)
-                          : launch_few_heads<kF16>(a, p.row_tiles, groups, st);
-  if (rc != SARATHI_OK || !cut) return rc;
-  return dtype == kBF16 ? launch_join<kBF16>(a, 16 * p.row_tiles, st)
-                        : launch_join<kF16>(a, 16 * p.row_tiles, st);
+  char* ws = workspace && aligned16(workspace) && workspace_bytes >= p.few.bytes() + p.tile.bytes()
+                 ? reinterpret_cast<char*>(workspace)
+                 : nullptr;
+  int rc = run_class(a, p.tile, ws, dtype, st, [&](const PagedAttnArgs& x, int64_t groups) {
+    return launch_attn_tiles(x, dtype, p.tile.rows, groups, st);
+  });
+  if (rc != SARATHI_OK) return rc;
+  return run_class(a, p.few, ws ? ws + p.tile.bytes() : nullptr, dtype, st,
+                   [&](const PagedAttnArgs& x, int64_t groups) {
+                     return dtype == kBF16 ? launch_few_heads<kBF16>(x, p.few.rows / 16, groups, st)
+                                           : launch_few_heads<kF16>(x, p.few.rows / 16, groups, st);
+                   });
 }

@@ -114,6 +114,12 @@ SK_DEV uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
   return v;
 }
 
+// Most keys that a tile of the request spans with a window, counted from a multiple of 64.
+SK_DEV int32_t attn_window_keys(const PagedAttnArgs& a, const AttnSeq& x) {
+  const int64_t s = (int64_t)a.window + x.n + 63;
+  return s < x.s ? (int32_t)s : x.s;
+}
+
 // Rows per tile ROWS, WAVES waves in the workgroup.  `want` counts the items of one key head in
 // the order request, tile, part.  Two sums over the requests: keys times tiles, which fixes the
 // part length (the same for all, at least min_part, a multiple of 64, so that about a.target
@@ -141,7 +147,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     for (int32_t r = r0; r < r1; ++r) {
       const AttnSeq x = attn_seq(a, r);
       int32_t s = x.s;  // keys that the tiles of this request walk, roughly
-      if (a.window >= 0 && s > a.window + x.n) s = a.window + x.n;
+      if (a.window >= 0) s = attn_window_keys(a, x);
       work += (uint64_t)tiles_of(x) * (uint32_t)s;
     }
     work = wave_scan_u64(work, lane);
@@ -157,8 +163,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     __syncthreads();  // sums[] is written again below
   }
   auto parts_of = [&](const AttnSeq& x) {
-    int32_t s = x.s;
-    if (a.window >= 0 && s > a.window + x.n) s = a.window + x.n;
+    const int32_t s = a.window >= 0 ? attn_window_keys(a, x) : x.s;
     return part_len == 0x7fffffff || s <= part_len ? 1 : (s - 1) / part_len + 1;
   };
   uint64_t mine = 0;
@@ -250,6 +255,32 @@ template <int BYTES> SK_DEV void dma_to_lds(const void* src, lds_char* base) {
   else
     __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 4, 0, 0);
 }
+
+// The same read for one address, its wait placed by the compiler; for kernels whose loads into LDS
+// are the ones below, of which the compiler knows nothing.
+SK_DEV u32x2 lds_read_tr_b64(const lds_char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)p));
+}
+// dma_to_lds() as instructions that the compiler does not look into: it places no waits for them, so
+// every read of what they bring stands behind a counted wait_vmcnt() (and a barrier, where another
+// wave loaded it).  No register is written but M0, which nothing else in those kernels uses.
+SK_DEV void dma_asm16(const void* src, lds_char* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr(base)), "v"(src)
+               : "memory");
+}
+SK_DEV void dma_asm16(const char* uniform_base, uint32_t off, lds_char* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr(base)), "v"(off),
+               "s"(uniform_base)
+               : "memory");
+}
+SK_DEV void dma_asm4(const void* src, lds_char* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr(base)), "v"(src)
+               : "memory");
+}
+// Meets the other waves; only LDS reads of this wave have to be complete (they are: their results
+// have been used).
+SK_DEV void wave_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Maximum / sum over the lanes that differ in bits 4 and 5.
 SK_DEV float group_max(float v) {

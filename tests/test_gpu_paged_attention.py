@@ -166,3 +166,21 @@ def test_merge_matches_definition(ops, dev, dtype, states, tokens, heads, head_s
     dead = want_z == -torch.inf
     assert torch.equal(z.cpu() == -torch.inf, dead)
     assert bool(((z.cpu().double() - want_z).abs()[~dead] <= 1e-6 * want_z.abs()[~dead] + 1e-6).all())
+
+
+@pytest.mark.parametrize("new,total", [
+    ([129], [129]), ([256], [900]), ([130, 1, 77, 1], [130, 64, 500, 3]), ([300], [2111]),
+    ([65, 64, 63, 1], [65, 640, 63, 1000]),
+])
+@pytest.mark.parametrize("heads,kv_heads,head_size,page_size,dtype", [
+    (8, 2, 128, 16, torch.bfloat16),
+    (4, 4, 128, 7, torch.float16),
+    (7, 1, 64, 32, torch.bfloat16),
+    (3, 1, 96, 16, torch.float16),
+    (2, 2, 40, 48, torch.bfloat16),
+])
+def test_chunks_match_definition(ops, dev, new, total, heads, kv_heads, head_size, page_size, dtype):
+    b = build_batch(11, page_size, new, total, heads, kv_heads, head_size, dtype)
+    for kw in (dict(), dict(causal=False), dict(window_left=100)):
+        got, lse = call(ops, dev, b, return_lse=True, **kw)
+        check(b, got, lse, reference(b, kw.get("causal", True), kw.get("window_left", -1)))
