@@ -57,12 +57,13 @@ constexpr float kRaise = 8.f;          // see "maximum" above
 
 SK_DEV void fence_order() { __builtin_amdgcn_sched_barrier(0); }
 
-template <int DT, int DP, int QT, bool PAD>
+// PAGE16: pages of a multiple of 16 keys, so that a wave's share of a step lies in one page.
+template <int DT, int DP, int QT, bool PAD, bool PAGE16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, QT == 2 ? 1 : 2)))
 void paged_attn_tile_kernel(PagedAttnArgs a) {
   using Sh = TileShape<DP>;
   constexpr int ROWS = 128 * QT, KSTEPS = DP / 16, DTILES = DP / 32;
-  constexpr int kOps = 2 * Sh::kDmas + 1;
+  constexpr int kOps = 2 * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads that a step asks for
   extern __shared__ u32x4 tile_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
   const AttnItem it = attn_find_item<ROWS, 4>(a, blockIdx.x / (uint32_t)a.kv_heads,
@@ -78,17 +79,16 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   const int32_t rows = rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
 
   u32x4 q[QT][KSTEPS];
-  int32_t lo[QT], hi[QT], tok[QT], head[QT];
+  int32_t row_tok[QT];  // token of this lane's row, counted from the request's first new one
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int32_t i = (wave * QT + qt) * 32 + col;
     const int32_t p = row0 + (i < rows ? i : rows - 1);
     const int32_t j = p / a.group;
-    tok[qt] = x.q0 + j;
-    head[qt] = (int32_t)h * a.group + (p - j * a.group);
-    attn_span(a, x, j, lo[qt], hi[qt]);
+    row_tok[qt] = j;
+    const int32_t head = (int32_t)h * a.group + (p - j * a.group);
     const char* src = reinterpret_cast<const char*>(a.q) +
-                      ((int64_t)tok[qt] * a.q_stride + (int64_t)head[qt] * a.head_size) * 2;
+                      ((int64_t)(x.q0 + j) * a.q_stride + (int64_t)head * a.head_size) * 2;
 #pragma unroll
     for (int k = 0; k < KSTEPS; ++k) {
       const int d = k * 16 + half * 8;
@@ -145,65 +145,93 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   // ---- loads: wave w brings keys 16 w .. 16 w + 15 of a step
   const char* const kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)h * a.head_size * 2;
   const char* const vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)h * a.head_size * 2;
-  const bool paged16 = a.page_size % 16 == 0 && a.entry_stride < (1 << 26);  // 32-bit offsets reach
-  int koff[Sh::kDmas], voff[Sh::kDmas];  // this lane's chunk of each load instruction
-  uint32_t erow[Sh::kDmas];              // row of that chunk times the entry stride
-#pragma unroll
-  for (int n = 0; n < Sh::kDmas; ++n) {
-    const int row = n * Sh::kRowsPerDma + lane / Sh::kChunks, pos = lane % Sh::kChunks;
-    koff[n] = (pos ^ Sh::swz_k(row)) * 16;  // 16 keys per wave: the swizzles depend on row % 16
-    voff[n] = (pos ^ Sh::swz_v(row)) * 16;
-    erow[n] = (uint32_t)row * (uint32_t)a.entry_stride;
-  }
+  // this lane's chunk of load instruction n: row n * kRowsPerDma + row_l of the share; the swizzle
+  // of K gains 4 n chunks from one instruction to the next, that of V nothing
+  const int row_l = lane / Sh::kChunks;
+  const uint32_t kchunk = (uint32_t)((lane % Sh::kChunks) ^ Sh::swz_k(row_l)) * 16u;
+  const uint32_t vchunk = (uint32_t)((lane % Sh::kChunks) ^ Sh::swz_v(row_l)) * 16u;
+  const uint32_t erow_l = (uint32_t)row_l * (uint32_t)a.entry_stride;
+  auto chunk_of = [&](bool keys, int n) { return keys ? kchunk ^ (uint32_t)(n * 64) : vchunk; };
+  auto share_at = [&](int32_t j) { return begin + j * 64 + wave * 16; };
+  auto clamp_key = [&](int32_t t) { return t < first ? first : t < end ? t : end - 1; };
   auto load_ids = [&](int32_t j) {
-    int32_t t = begin + j * 64 + wave * 16 + (lane & 15);
-    t = t < first ? first : t < end ? t : end - 1;
-    dma_asm4(a.kv_indices + x.kv0 + attn_page_of(a, t), ids + (j % Sh::kIdSlots) * 256);
+    if constexpr (!PAGE16)
+      dma_asm4(a.kv_indices + x.kv0 + attn_page_of(a, clamp_key(share_at(j) + (lane & 15))),
+               ids + (j % Sh::kIdSlots) * 256);
   };
-  auto load_share = [&](int32_t j, const char* cache, lds_char* dst, const int (&off)[Sh::kDmas]) {
-    const int32_t t0 = begin + j * 64 + wave * 16;
+  // PAGE16: the sixteen keys of share j, or of the nearest share that holds one of [first, end), and
+  // their page (a scalar load, used one step later)
+  auto share_base = [&](int32_t j) {
+    const int32_t t = share_at(j), t0 = first & ~15, t1 = (end - 1) & ~15;
+    return t < t0 ? t0 : t < t1 ? t : t1;
+  };
+  auto share_page = [&](int32_t j) {
+    return PAGE16 ? a.kv_indices[x.kv0 + attn_page_of(a, share_base(j))] : 0;
+  };
+  auto load_share = [&](int32_t j, int32_t page, const char* cache, bool keys, lds_char* dst) {
     lds_char* const at = dst + wave * (16 * Sh::kRowBytes);
-    int32_t page = *(const __attribute__((address_space(3))) int32_t*)(
-        ids + (j % Sh::kIdSlots) * 256 + (lane & 15) * 4);
-    page = attn_clip_page(a, page);
-    if (paged16 && t0 >= first && t0 + 16 <= end) {
-      page = __builtin_amdgcn_readfirstlane(page);
+    if constexpr (PAGE16) {
+      const int32_t t0 = share_base(j);
       const int32_t entry = t0 - attn_page_of(a, t0) * a.page_size;
-      const char* const base = cache + page * a.page_stride + entry * a.entry_stride;
+      const char* const base = cache + attn_clip_page(a, page) * a.page_stride + entry * a.entry_stride;
+      if (t0 >= first && t0 + 16 <= end) {
 #pragma unroll
-      for (int n = 0; n < Sh::kDmas; ++n)
-        if (!PAD || off[n] < a.head_size * 2) dma_asm16(base, erow[n] + off[n], at + n * 1024);
+        for (int n = 0; n < Sh::kDmas; ++n) {
+          const uint32_t c = chunk_of(keys, n);
+          if (!PAD || c < (uint32_t)a.head_size * 2u)
+            dma_asm16(base + n * Sh::kRowsPerDma * a.entry_stride, erow_l + c, at + n * 1024);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < Sh::kDmas; ++n) {
+          const uint32_t c = chunk_of(keys, n);
+          const int32_t row = clamp_key(t0 + n * Sh::kRowsPerDma + row_l) - t0;
+          if (!PAD || c < (uint32_t)a.head_size * 2u)
+            dma_asm16(base, (uint32_t)row * (uint32_t)a.entry_stride + c, at + n * 1024);
+        }
+      }
     } else {
-      int32_t t = t0 + (lane & 15);
-      t = t < first ? first : t < end ? t : end - 1;
-      const int64_t e = page * a.page_stride + (int64_t)(t - attn_page_of(a, t) * a.page_size) * a.entry_stride;
+      const int32_t t = clamp_key(share_at(j) + (lane & 15));
+      page = *(const __attribute__((address_space(3))) int32_t*)(
+          ids + (j % Sh::kIdSlots) * 256 + (lane & 15) * 4);
+      const int64_t e = attn_clip_page(a, page) * a.page_stride +
+                        (int64_t)(t - attn_page_of(a, t) * a.page_size) * a.entry_stride;
       const int32_t e_lo = (int32_t)e, e_hi = (int32_t)(e >> 32);
 #pragma unroll
       for (int n = 0; n < Sh::kDmas; ++n) {
-        const int row = n * Sh::kRowsPerDma + lane / Sh::kChunks;
+        const int row = n * Sh::kRowsPerDma + row_l;
         const int64_t s = (int64_t)(((uint64_t)(uint32_t)__shfl(e_hi, row, 64) << 32) |
                                     (uint32_t)__shfl(e_lo, row, 64));
-        if (!PAD || off[n] < a.head_size * 2) dma_asm16(cache + s + off[n], at + n * 1024);
+        const uint32_t c = chunk_of(keys, n);
+        if (!PAD || c < (uint32_t)a.head_size * 2u) dma_asm16(cache + s + c, at + n * 1024);
       }
     }
   };
-  auto load_k = [&](int32_t j) { load_share(j, kc, klds + (uint32_t)j % Sh::kKeySteps * Sh::kStepBytes, koff); };
-  auto load_v = [&](int32_t j) { load_share(j, vc, vlds + (uint32_t)j % Sh::kValueSteps * Sh::kStepBytes, voff); };
+  auto load_k = [&](int32_t j, int32_t page) {
+    load_share(j, page, kc, true, klds + (uint32_t)j % Sh::kKeySteps * Sh::kStepBytes);
+  };
+  auto load_v = [&](int32_t j, int32_t page) {
+    load_share(j, page, vc, false, vlds + (uint32_t)j % Sh::kValueSteps * Sh::kStepBytes);
+  };
 
   // ---- operand reads
-  const lds_char* const kread = klds + col * Sh::kRowBytes;
-  auto read_k = [&](int32_t u, int k) {
-    return *(const __attribute__((address_space(3))) u32x4*)(
-        kread + (uint32_t)u / 2 % Sh::kKeySteps * Sh::kStepBytes + (u & 1) * 32 * Sh::kRowBytes +
-        (((k * 2 + half) ^ Sh::swz_k(col)) * 16));
-  };
+  uint32_t kread[KSTEPS], vread[DTILES];
+#pragma unroll
+  for (int k = 0; k < KSTEPS; ++k)
+    kread[k] = lds_addr(klds) + col * Sh::kRowBytes + (((k * 2 + half) ^ Sh::swz_k(col)) * 16);
   const int vlane = lane & 15, vrow = half * 4 + (vlane >> 2);
-  const lds_char* const vread = vlds + vrow * Sh::kRowBytes + (vlane & 1) * 8;
-  auto read_v = [&](int32_t u, int ks, int dt) {  // ks: 16 of the 32 keys
+#pragma unroll
+  for (int dt = 0; dt < DTILES; ++dt) {
     const int chunk = dt * 4 + ((lane >> 4) & 1) * 2 + ((vlane >> 1) & 1);
-    const lds_char* const p = vread + (uint32_t)u / 2 % Sh::kValueSteps * Sh::kStepBytes +
-                              ((u & 1) * 32 + ks * 16) * Sh::kRowBytes +
-                              ((chunk ^ Sh::swz_v(vrow)) * 16);
+    vread[dt] = lds_addr(vlds) + vrow * Sh::kRowBytes + (chunk ^ Sh::swz_v(vrow)) * 16 + (vlane & 1) * 8;
+  }
+  auto read_k = [&](uint32_t step_at, int sub, int k) {
+    return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)(
+        kread[k] + step_at + sub * (32 * Sh::kRowBytes));
+  };
+  auto read_v = [&](uint32_t step_at, int sub, int ks, int dt) {  // ks: 16 of the 32 keys
+    const lds_char* const p = (const lds_char*)(uintptr_t)(vread[dt] + step_at) +
+                              (sub * 32 + ks * 16) * Sh::kRowBytes;
     const u32x2 x0 = lds_read_tr_b64(p), x1 = lds_read_tr_b64(p + 8 * Sh::kRowBytes);
     return u32x4{x0[0], x0[1], x1[0], x1[1]};
   };
@@ -215,7 +243,9 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     if (t0 >= full_lo && t0 + 32 <= full_hi && t0 + 32 <= end) return;  // uniform over the wave
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int32_t top = (hi[qt] < end ? hi[qt] : end) - t0 - 4 * half, low = lo[qt] - t0 - 4 * half;
+      int32_t lo, hi;
+      attn_span(a, x, row_tok[qt], lo, hi);
+      const int32_t top = (hi < end ? hi : end) - t0 - 4 * half, low = lo - t0 - 4 * half;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int32_t t = 8 * (i / 4) + i % 4;
@@ -246,8 +276,11 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   };
   // The scores of keys u become probabilities and meet the values, while (MORE) those of keys u + 1
   // are formed and their maximum is taken.
-  auto body = [&](int32_t u, Scores& cur, Scores& next, auto more) {
+  auto body = [&](int32_t u, auto sub, Scores& cur, Scores& next, auto more) {
     constexpr bool MORE = decltype(more)::value;
+    constexpr int SUB = decltype(sub)::value;  // u & 1
+    const uint32_t v_at = (uint32_t)u / 2 % Sh::kValueSteps * Sh::kStepBytes;
+    const uint32_t k_at = ((uint32_t)u + 1) / 2 % Sh::kKeySteps * Sh::kStepBytes;
     constexpr int PER = QT * 16 / KSTEPS;  // probabilities per operand of the next scores
     constexpr int PV = 2 * DTILES;         // operands of the output's products
     constexpr int PERM = QT * 16 / PV;     // scores that enter the maximum per such operand
@@ -257,19 +290,19 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
       for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) next.s[qt][i] = 0.f;
-      kf[0] = read_k(u + 1, 0);
-      kf[1] = read_k(u + 1, 1);
+      kf[0] = read_k(k_at, SUB ^ 1, 0);
+      kf[1] = read_k(k_at, SUB ^ 1, 1);
     }
 #pragma unroll
     for (int n = 0; n < KSTEPS; ++n) {
       if constexpr (MORE) {
-        if (n + 2 < KSTEPS) kf[(n + 2) % 3] = read_k(u + 1, n + 2);
+        if (n + 2 < KSTEPS) kf[(n + 2) % 3] = read_k(k_at, SUB ^ 1, n + 2);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
           next.s[qt] = mfma32x16<DT>(kf[n % 3], q[qt][n], next.s[qt]);
       }
-      if (n == KSTEPS - 2) vf[0] = read_v(u, 0, 0);
-      if (n == KSTEPS - 1) vf[1] = read_v(u, 0, 1);
+      if (n == KSTEPS - 2) vf[0] = read_v(v_at, SUB, 0, 0);
+      if (n == KSTEPS - 1) vf[1] = read_v(v_at, SUB, 0, 1);
 #pragma unroll
       for (int e = n * PER; e < (n + 1) * PER; e += 2) {
         const int qt = e / 16, i = e % 16;
@@ -277,7 +310,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
         const float z1 = __builtin_amdgcn_exp2f(fmaf(cur.s[qt][i + 1], a.scale_log2, -ref[qt]));
         l[qt] += z0 + z1;
         uint32_t w = pack2<DT>(z0, z1);
-        asm volatile("" : "+v"(w));  // made here, not where it is used
+        asm volatile("" : "+v"(w), "+v"(l[qt]));  // made here, not where they are used
         p[qt][i / 8][i / 2 % 4] = w;
       }
       fence_order();
@@ -288,7 +321,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     for (int qt = 0; qt < QT; ++qt) top[qt] = -INFINITY;
 #pragma unroll
     for (int n = 0; n < PV; ++n) {
-      if (n + 2 < PV) vf[(n + 2) % 3] = read_v(u, (n + 2) / DTILES, (n + 2) % DTILES);
+      if (n + 2 < PV) vf[(n + 2) % 3] = read_v(v_at, SUB, (n + 2) / DTILES, (n + 2) % DTILES);
       const int ks = n / DTILES, dt = n % DTILES;
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) o[dt][qt] = mfma32x16<DT>(vf[n % 3], p[qt][ks], o[dt][qt]);
@@ -305,14 +338,21 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   };
 
   if (steps > 0) {
+    if constexpr (!PAGE16) {
 #pragma unroll
-    for (int i = 0; i < 6; ++i) load_ids(i);
-    wait_vmcnt<0>();
-    load_k(0);
-    load_k(1);
-    load_v(0);
-    load_k(2);
-    load_v(1);
+      for (int i = 0; i < 6; ++i) load_ids(i);
+      wait_vmcnt<0>();
+    }
+    // pages of the steps whose keys, resp. values, are asked for next
+    int32_t page_v = share_page(2), page_k = share_page(3);
+    {
+      const int32_t p0 = share_page(0), p1 = share_page(1);
+      load_k(0, p0);
+      load_k(1, p1);
+      load_v(0, p0);
+      load_k(2, page_v);
+      load_v(1, p1);
+    }
     wait_vmcnt<4 * Sh::kDmas>();  // keys of step 0
     wave_barrier();
     Scores s0, s1;
@@ -324,7 +364,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
         for (int i = 0; i < 16; ++i) s0.s[qt][i] = 0.f;
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        const u32x4 kk = read_k(0, k);
+        const u32x4 kk = read_k(0, 0, k);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) s0.s[qt] = mfma32x16<DT>(kk, q[qt][k], s0.s[qt]);
       }
@@ -337,7 +377,11 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
       }
       raise(top);
     }
-    auto turn = [&](int32_t j) {
+    // Step j: keys j + 1 and values j have landed once only what step j - 1 asked for is missing
+    // (before the first: keys 2 and values 1).
+    int32_t j = 0;
+    wait_vmcnt<2 * Sh::kDmas>();
+    while (j + 1 < steps) {
       // the register file's two halves: the output in the accumulators, everything else beside it
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
@@ -347,24 +391,19 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
         for (int k = 0; k < KSTEPS; ++k) asm volatile("" : "+v"(q[qt][k]));
       }
       wave_barrier();
-      load_k(j + 3);
-      load_v(j + 2);
+      load_k(j + 3, page_k);
+      load_v(j + 2, page_v);
       load_ids(j + 6);
-    };
-    // before step j: keys j + 1 and values j have landed once only what step j - 1 asked for is
-    // missing (before the first: keys 2 and values 1)
-    int32_t j = 0;
-    wait_vmcnt<2 * Sh::kDmas>();
-    while (j + 1 < steps) {
-      turn(j);
-      body(2 * j, s0, s1, std::true_type{});
-      body(2 * j + 1, s1, s0, std::true_type{});
+      page_v = page_k;
+      page_k = share_page(j + 4);
+      body(2 * j, std::integral_constant<int, 0>{}, s0, s1, std::true_type{});
+      body(2 * j + 1, std::integral_constant<int, 1>{}, s1, s0, std::true_type{});
       wait_vmcnt<kOps>();
       ++j;
     }
     wave_barrier();
-    body(2 * j, s0, s1, std::true_type{});
-    body(2 * j + 1, s1, s0, std::false_type{});
+    body(2 * j, std::integral_constant<int, 0>{}, s0, s1, std::true_type{});
+    body(2 * j + 1, std::integral_constant<int, 1>{}, s1, s0, std::false_type{});
     wait_vmcnt<0>();  // nothing may land in LDS after this workgroup has left it
   }
 
@@ -394,8 +433,10 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
         }
     } else {
       const float inv = l[qt] == 0.f ? 0.f : 1.f / l[qt];
+      const int64_t tok = x.q0 + row_tok[qt];
+      const int32_t head = (int32_t)h * a.group + (row0 + i - row_tok[qt] * a.group);
       char* const dst = reinterpret_cast<char*>(a.out) +
-                        ((int64_t)tok[qt] * a.out_stride + (int64_t)head[qt] * a.head_size) * 2;
+                        (tok * a.out_stride + (int64_t)head * a.head_size) * 2;
 #pragma unroll
       for (int dt = 0; dt < DTILES; ++dt)
 #pragma unroll
@@ -407,23 +448,28 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
                       pack2<DT>(o[dt][qt][b * 4 + 2] * inv, o[dt][qt][b * 4 + 3] * inv)};
         }
       if (a.lse && half == 0)
-        a.lse[(int64_t)tok[qt] * a.heads + head[qt]] = attn_lse(ref[qt], l[qt]);
+        a.lse[tok * a.heads + head] = attn_lse(ref[qt], l[qt]);
     }
   }
 }
 
+template <int DT, int DP, int QT, bool PAD, bool PAGE16>
+static int launch_tile_pages(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
+  constexpr int bytes = TileShape<DP>::kBytes;
+  if (!allow_lds<paged_attn_tile_kernel<DT, DP, QT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
+  hipLaunchKernelGGL((paged_attn_tile_kernel<DT, DP, QT, PAD, PAGE16>), dim3((unsigned)groups),
+                     dim3(256), bytes, st, a);
+  return launch_status();
+}
 template <int DT, int DP, int QT>
 static int launch_tile(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
-  constexpr int bytes = TileShape<DP>::kBytes;
-  const dim3 grid((unsigned)groups), block(256);
-  if (a.head_size == DP) {
-    if (!allow_lds<paged_attn_tile_kernel<DT, DP, QT, false>>(bytes)) return SARATHI_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_attn_tile_kernel<DT, DP, QT, false>), grid, block, bytes, st, a);
-  } else {
-    if (!allow_lds<paged_attn_tile_kernel<DT, DP, QT, true>>(bytes)) return SARATHI_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_attn_tile_kernel<DT, DP, QT, true>), grid, block, bytes, st, a);
-  }
-  return launch_status();
+  // offsets inside a share are 32-bit
+  const bool page16 = a.page_size % 16 == 0 && a.entry_stride < (1 << 26);
+  if (a.head_size == DP)
+    return page16 ? launch_tile_pages<DT, DP, QT, false, true>(a, groups, st)
+                  : launch_tile_pages<DT, DP, QT, false, false>(a, groups, st);
+  return page16 ? launch_tile_pages<DT, DP, QT, true, true>(a, groups, st)
+                : launch_tile_pages<DT, DP, QT, true, false>(a, groups, st);
 }
 template <int DT>
 static int launch_tile_heads(const PagedAttnArgs& a, int rows, int64_t groups, hipStream_t st) {
