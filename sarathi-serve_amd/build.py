@@ -43,6 +43,9 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=16",
     "-Wall", "-Wno-unused-command-line-argument",
 ]
+# Per source: the tile kernel of the attention wants the results of its matrix instructions in
+# registers that the vector unit can read (its softmax works on them).
+SOURCE_FLAGS = {"paged_attention_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # extra hipcc flags for tuning builds, e.g. -DSARATHI_KV_STORE_POLICY=18
 HIP_FLAGS += os.environ.get("SARATHI_HIPCC_EXTRA_FLAGS", "").split()
 
@@ -66,7 +69,7 @@ def build_abi_library(verbose=False, jobs=8):
     for src in HIP_SOURCES + CXX_SOURCES:
         obj = os.path.join(OBJ_DIR, src + ".o")
         objs.append(obj)
-        cmds.append([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj])
+        cmds.append([HIPCC] + HIP_FLAGS + SOURCE_FLAGS.get(src, []) + ["-c", os.path.join(CSRC, src), "-o", obj])
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
         list(pool.map(lambda c: _run(c, verbose), cmds))
     _run([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", ABI_LIB] + objs, verbose)

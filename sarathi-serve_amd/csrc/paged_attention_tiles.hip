@@ -47,7 +47,7 @@ template <int DP> struct TileShape {
   static constexpr int kStepBytes = 64 * kRowBytes;
   static constexpr int kIdSlots = 8;
   static constexpr int kRingBytes = (kKeySteps + kValueSteps) * kStepBytes;
-  static constexpr int kBytes = kRingBytes + 4 * kIdSlots * 256;
+  static constexpr int kBytes = kRingBytes + 8 * kIdSlots * 256;
   SK_DEV static int swz_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
   SK_DEV static int swz_v(int row) { return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 };
@@ -58,19 +58,22 @@ constexpr float kRaise = 8.f;          // see "maximum" above
 SK_DEV void fence_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // PAGE16: pages of a multiple of 16 keys, so that a wave's share of a step lies in one page.
-template <int DT, int DP, int QT, bool PAD, bool PAGE16>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, QT == 2 ? 1 : 2)))
+template <int DT, int DP, int WAVES, int QT, bool PAD, bool PAGE16>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4)))
 void paged_attn_tile_kernel(PagedAttnArgs a) {
   using Sh = TileShape<DP>;
-  constexpr int ROWS = 128 * QT, KSTEPS = DP / 16, DTILES = DP / 32;
-  constexpr int kOps = 2 * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads that a step asks for
+  constexpr int ROWS = WAVES * 32 * QT, KSTEPS = DP / 16, DTILES = DP / 32;
+  constexpr int kSteps = WAVES == 8 ? 1 : 2;      // 8 waves: half of them bring keys, half values
+  constexpr int kOps = kSteps * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads that a step asks for
   extern __shared__ u32x4 tile_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
-  const AttnItem it = attn_find_item<ROWS, 4>(a, blockIdx.x / (uint32_t)a.kv_heads,
+  const AttnItem it = attn_find_item<ROWS, WAVES>(a, blockIdx.x / (uint32_t)a.kv_heads,
                                               a.part_map != nullptr && blockIdx.x == 0);
   if (it.r < 0) return;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int share = wave & 3;
+  const bool brings_k = WAVES == 4 || wave < 4, brings_v = WAVES == 4 || wave >= 4;
   const AttnSeq x = attn_seq(a, it.r);
   const int32_t rows_all = x.n * a.group;
   const int32_t tiles = (rows_all + ROWS - 1) / ROWS;
@@ -137,7 +140,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   lds_char* const vlds = lds + Sh::kKeySteps * Sh::kStepBytes;
   lds_char* const ids = lds + Sh::kRingBytes + wave * (Sh::kIdSlots * 256);
   if constexpr (PAD) {  // chunks beyond the head are never loaded: they stay zero
-    for (int i = tid * 16; i < Sh::kRingBytes; i += 4096)
+    for (int i = tid * 16; i < Sh::kRingBytes; i += WAVES * 1024)
       *(__attribute__((address_space(3))) u32x4*)(lds + i) = u32x4{0, 0, 0, 0};
     __syncthreads();
   }
@@ -152,7 +155,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   const uint32_t vchunk = (uint32_t)((lane % Sh::kChunks) ^ Sh::swz_v(row_l)) * 16u;
   const uint32_t erow_l = (uint32_t)row_l * (uint32_t)a.entry_stride;
   auto chunk_of = [&](bool keys, int n) { return keys ? kchunk ^ (uint32_t)(n * 64) : vchunk; };
-  auto share_at = [&](int32_t j) { return begin + j * 64 + wave * 16; };
+  auto share_at = [&](int32_t j) { return begin + j * 64 + share * 16; };
   auto clamp_key = [&](int32_t t) { return t < first ? first : t < end ? t : end - 1; };
   auto load_ids = [&](int32_t j) {
     if constexpr (!PAGE16)
@@ -169,7 +172,7 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     return PAGE16 ? a.kv_indices[x.kv0 + attn_page_of(a, share_base(j))] : 0;
   };
   auto load_share = [&](int32_t j, int32_t page, const char* cache, bool keys, lds_char* dst) {
-    lds_char* const at = dst + wave * (16 * Sh::kRowBytes);
+    lds_char* const at = dst + share * (16 * Sh::kRowBytes);
     if constexpr (PAGE16) {
       const int32_t t0 = share_base(j);
       const int32_t entry = t0 - attn_page_of(a, t0) * a.page_size;
@@ -208,10 +211,10 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     }
   };
   auto load_k = [&](int32_t j, int32_t page) {
-    load_share(j, page, kc, true, klds + (uint32_t)j % Sh::kKeySteps * Sh::kStepBytes);
+    if (brings_k) load_share(j, page, kc, true, klds + (uint32_t)j % Sh::kKeySteps * Sh::kStepBytes);
   };
   auto load_v = [&](int32_t j, int32_t page) {
-    load_share(j, page, vc, false, vlds + (uint32_t)j % Sh::kValueSteps * Sh::kStepBytes);
+    if (brings_v) load_share(j, page, vc, false, vlds + (uint32_t)j % Sh::kValueSteps * Sh::kStepBytes);
   };
 
   // ---- operand reads
@@ -353,7 +356,8 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
       load_k(2, page_v);
       load_v(1, p1);
     }
-    wait_vmcnt<4 * Sh::kDmas>();  // keys of step 0
+    // keys of step 0 (8 waves: steps 0 and 1 are all that a wave has asked for besides keys 2)
+    if constexpr (WAVES == 4) wait_vmcnt<4 * Sh::kDmas>(); else wait_vmcnt<Sh::kDmas>();
     wave_barrier();
     Scores s0, s1;
     {
@@ -380,16 +384,8 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     // Step j: keys j + 1 and values j have landed once only what step j - 1 asked for is missing
     // (before the first: keys 2 and values 1).
     int32_t j = 0;
-    wait_vmcnt<2 * Sh::kDmas>();
+    if constexpr (WAVES == 4) wait_vmcnt<2 * Sh::kDmas>(); else wait_vmcnt<0>();
     while (j + 1 < steps) {
-      // the register file's two halves: the output in the accumulators, everything else beside it
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-#pragma unroll
-        for (int dt = 0; dt < DTILES; ++dt) asm volatile("" : "+a"(o[dt][qt]));
-#pragma unroll
-        for (int k = 0; k < KSTEPS; ++k) asm volatile("" : "+v"(q[qt][k]));
-      }
       wave_barrier();
       load_k(j + 3, page_k);
       load_v(j + 2, page_v);
@@ -453,29 +449,29 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   }
 }
 
-template <int DT, int DP, int QT, bool PAD, bool PAGE16>
+template <int DT, int DP, int WAVES, int QT, bool PAD, bool PAGE16>
 static int launch_tile_pages(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
   constexpr int bytes = TileShape<DP>::kBytes;
-  if (!allow_lds<paged_attn_tile_kernel<DT, DP, QT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
-  hipLaunchKernelGGL((paged_attn_tile_kernel<DT, DP, QT, PAD, PAGE16>), dim3((unsigned)groups),
-                     dim3(256), bytes, st, a);
+  if (!allow_lds<paged_attn_tile_kernel<DT, DP, WAVES, QT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
+  hipLaunchKernelGGL((paged_attn_tile_kernel<DT, DP, WAVES, QT, PAD, PAGE16>), dim3((unsigned)groups),
+                     dim3(WAVES * 64), bytes, st, a);
   return launch_status();
 }
-template <int DT, int DP, int QT>
+template <int DT, int DP, int WAVES, int QT>
 static int launch_tile(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
   // offsets inside a share are 32-bit
   const bool page16 = a.page_size % 16 == 0 && a.entry_stride < (1 << 26);
   if (a.head_size == DP)
-    return page16 ? launch_tile_pages<DT, DP, QT, false, true>(a, groups, st)
-                  : launch_tile_pages<DT, DP, QT, false, false>(a, groups, st);
-  return page16 ? launch_tile_pages<DT, DP, QT, true, true>(a, groups, st)
-                : launch_tile_pages<DT, DP, QT, true, false>(a, groups, st);
+    return page16 ? launch_tile_pages<DT, DP, WAVES, QT, false, true>(a, groups, st)
+                  : launch_tile_pages<DT, DP, WAVES, QT, false, false>(a, groups, st);
+  return page16 ? launch_tile_pages<DT, DP, WAVES, QT, true, true>(a, groups, st)
+                : launch_tile_pages<DT, DP, WAVES, QT, true, false>(a, groups, st);
 }
 template <int DT>
 static int launch_tile_heads(const PagedAttnArgs& a, int rows, int64_t groups, hipStream_t st) {
   if (a.head_size <= 64)
-    return rows == 256 ? launch_tile<DT, 64, 2>(a, groups, st) : launch_tile<DT, 64, 1>(a, groups, st);
-  return rows == 256 ? launch_tile<DT, 128, 2>(a, groups, st) : launch_tile<DT, 128, 1>(a, groups, st);
+    return rows == 256 ? launch_tile<DT, 64, 8, 1>(a, groups, st) : launch_tile<DT, 64, 4, 1>(a, groups, st);
+  return rows == 256 ? launch_tile<DT, 128, 8, 1>(a, groups, st) : launch_tile<DT, 128, 4, 1>(a, groups, st);
 }
 
 int launch_attn_tiles(const PagedAttnArgs& a, int dtype, int rows, int64_t groups, hipStream_t st) {
