@@ -601,8 +601,8 @@ extern "C" int sarathi_paged_attention(
   a.entry_stride = entry_stride * 2;
   int up = 0;
   while (((int64_t)1 << up) < page_size) ++up;
-  a.page_shift = 31 + up;  // exact for positions below 2^31
-  a.page_magic = (((uint64_t)1 << a.page_shift) + page_size - 1) / page_size;
+  a.page_shift = 31 + up;  // exact for positions below 2^31, and the factor stays below 2^32
+  a.page_magic = (uint32_t)((((uint64_t)1 << a.page_shift) + page_size - 1) / page_size);
   a.seqs = (int32_t)num_seqs;
   a.tokens = (int32_t)num_tokens;
   a.heads = num_heads;

@@ -43,11 +43,11 @@ template <int DP> struct TileShape {
   static constexpr int kChunks = DP / 8;
   static constexpr int kRowsPerDma = 64 / kChunks;
   static constexpr int kDmas = 16 / kRowsPerDma;  // a wave's 16 keys (or values) of a step
-  static constexpr int kKeySteps = 4, kValueSteps = 3;  // in LDS at a time
+  static constexpr int kSteps = 4;                // of keys, and of values, in LDS at a time
   static constexpr int kStepBytes = 64 * kRowBytes;
   static constexpr int kIdSlots = 8;
-  static constexpr int kRingBytes = (kKeySteps + kValueSteps) * kStepBytes;
-  static constexpr int kBytes = kRingBytes + 8 * kIdSlots * 256;
+  static constexpr int kRingBytes = 2 * kSteps * kStepBytes;
+  static constexpr int kBytes = kRingBytes + 8 * kIdSlots * 64;
   SK_DEV static int swz_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
   SK_DEV static int swz_v(int row) { return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 };
@@ -63,8 +63,9 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVE
 void paged_attn_tile_kernel(PagedAttnArgs a) {
   using Sh = TileShape<DP>;
   constexpr int ROWS = WAVES * 32 * QT, KSTEPS = DP / 16, DTILES = DP / 32;
-  constexpr int kSteps = WAVES == 8 ? 1 : 2;      // 8 waves: half of them bring keys, half values
-  constexpr int kOps = kSteps * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads that a step asks for
+  constexpr int ROLES = WAVES == 8 ? 1 : 2;  // 8 waves: half of them bring keys, half values
+  constexpr int kOps = ROLES * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads a wave issues per step
+  constexpr int AHEAD = 3;                   // operands read from LDS before their products
   extern __shared__ u32x4 tile_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
   const AttnItem it = attn_find_item<ROWS, WAVES>(a, blockIdx.x / (uint32_t)a.kv_heads,
@@ -73,7 +74,6 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int share = wave & 3;
-  const bool brings_k = WAVES == 4 || wave < 4, brings_v = WAVES == 4 || wave >= 4;
   const AttnSeq x = attn_seq(a, it.r);
   const int32_t rows_all = x.n * a.group;
   const int32_t tiles = (rows_all + ROWS - 1) / ROWS;
@@ -137,66 +137,81 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
 
   lds_char* const lds = (lds_char*)tile_lds;
   lds_char* const klds = lds;
-  lds_char* const vlds = lds + Sh::kKeySteps * Sh::kStepBytes;
-  lds_char* const ids = lds + Sh::kRingBytes + wave * (Sh::kIdSlots * 256);
+  lds_char* const vlds = lds + Sh::kSteps * Sh::kStepBytes;
+  lds_char* const ids = lds + Sh::kRingBytes + wave * (Sh::kIdSlots * 64);
   if constexpr (PAD) {  // chunks beyond the head are never loaded: they stay zero
     for (int i = tid * 16; i < Sh::kRingBytes; i += WAVES * 1024)
       *(__attribute__((address_space(3))) u32x4*)(lds + i) = u32x4{0, 0, 0, 0};
     __syncthreads();
   }
 
-  // ---- loads: wave w brings keys 16 w .. 16 w + 15 of a step
-  const char* const kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)h * a.head_size * 2;
-  const char* const vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)h * a.head_size * 2;
-  // this lane's chunk of load instruction n: row n * kRowsPerDma + row_l of the share; the swizzle
-  // of K gains 4 n chunks from one instruction to the next, that of V nothing
-  const int row_l = lane / Sh::kChunks;
-  const uint32_t kchunk = (uint32_t)((lane % Sh::kChunks) ^ Sh::swz_k(row_l)) * 16u;
-  const uint32_t vchunk = (uint32_t)((lane % Sh::kChunks) ^ Sh::swz_v(row_l)) * 16u;
-  const uint32_t erow_l = (uint32_t)row_l * (uint32_t)a.entry_stride;
-  auto chunk_of = [&](bool keys, int n) { return keys ? kchunk ^ (uint32_t)(n * 64) : vchunk; };
+  // ---- loads.  A share is sixteen keys or values of a step; a wave brings one share of each, or
+  // (8 waves) waves 0-3 bring keys and waves 4-7 values.
+  const char* src[ROLES];
+  lds_char* dst[ROLES];
+  uint32_t off[ROLES][Sh::kDmas];  // this lane's chunk of each load, from the share's first entry
+  const int row_l = lane / Sh::kChunks, pos_l = lane % Sh::kChunks;
+#pragma unroll
+  for (int r = 0; r < ROLES; ++r) {
+    const bool keys = ROLES == 2 ? r == 0 : wave < 4;
+    src[r] = reinterpret_cast<const char*>(keys ? a.k_cache : a.v_cache) + (int64_t)h * a.head_size * 2;
+    dst[r] = (keys ? klds : vlds) + share * (16 * Sh::kRowBytes);
+#pragma unroll
+    for (int n = 0; n < Sh::kDmas; ++n) {
+      const int row = n * Sh::kRowsPerDma + row_l;
+      off[r][n] = (uint32_t)(pos_l ^ (keys ? Sh::swz_k(row) : Sh::swz_v(row))) * 16u;
+      if constexpr (PAGE16) off[r][n] += (uint32_t)row * (uint32_t)a.entry_stride;
+    }
+  }
+  // chunk of off[r][n] inside the head's row
+  auto chunk_of = [&](int r, int n) {
+    return PAGE16 ? off[r][n] - (uint32_t)(n * Sh::kRowsPerDma + row_l) * (uint32_t)a.entry_stride
+                  : off[r][n];
+  };
   auto share_at = [&](int32_t j) { return begin + j * 64 + share * 16; };
   auto clamp_key = [&](int32_t t) { return t < first ? first : t < end ? t : end - 1; };
   auto load_ids = [&](int32_t j) {
-    if constexpr (!PAGE16)
-      dma_asm4(a.kv_indices + x.kv0 + attn_page_of(a, clamp_key(share_at(j) + (lane & 15))),
-               ids + (j % Sh::kIdSlots) * 256);
+    if constexpr (!PAGE16) {
+      const int32_t* const from = a.kv_indices + x.kv0 + attn_page_of(a, clamp_key(share_at(j) + (lane & 15)));
+      if (lane < 16) dma_asm4(from, ids + (j % Sh::kIdSlots) * 64);
+    }
   };
-  // PAGE16: the sixteen keys of share j, or of the nearest share that holds one of [first, end), and
-  // their page (a scalar load, used one step later)
-  auto share_base = [&](int32_t j) {
-    const int32_t t = share_at(j), t0 = first & ~15, t1 = (end - 1) & ~15;
-    return t < t0 ? t0 : t < t1 ? t : t1;
-  };
+  // PAGE16: the share of step j, or the nearest one that holds one of the keys [first, end), and its
+  // page number (a scalar load, used one step later)
+  const int32_t share_lo = first & ~15, share_hi = (end - 1) & ~15;
+  auto share_base = [&](int32_t j) { return clamp_i32(share_at(j), share_lo, share_hi); };
   auto share_page = [&](int32_t j) {
     return PAGE16 ? a.kv_indices[x.kv0 + attn_page_of(a, share_base(j))] : 0;
   };
-  auto load_share = [&](int32_t j, int32_t page, const char* cache, bool keys, lds_char* dst) {
-    lds_char* const at = dst + share * (16 * Sh::kRowBytes);
+  auto load_step = [&](int32_t j, int32_t page) {
+    const uint32_t slot = (uint32_t)j % Sh::kSteps * Sh::kStepBytes;
     if constexpr (PAGE16) {
       const int32_t t0 = share_base(j);
-      const int32_t entry = t0 - attn_page_of(a, t0) * a.page_size;
-      const char* const base = cache + attn_clip_page(a, page) * a.page_stride + entry * a.entry_stride;
-      if (t0 >= first && t0 + 16 <= end) {
+      const int64_t e = attn_clip_page(a, page) * a.page_stride +
+                        (int64_t)(t0 - attn_page_of(a, t0) * a.page_size) * a.entry_stride;
+      const bool inside = t0 >= first && t0 + 16 <= end;  // uniform over the wave
 #pragma unroll
-        for (int n = 0; n < Sh::kDmas; ++n) {
-          const uint32_t c = chunk_of(keys, n);
-          if (!PAD || c < (uint32_t)a.head_size * 2u)
-            dma_asm16(base + n * Sh::kRowsPerDma * a.entry_stride, erow_l + c, at + n * 1024);
-        }
-      } else {
+      for (int r = 0; r < ROLES; ++r) {
+        const char* const base = src[r] + e;
+        const uint32_t to = lds_addr(dst[r]) + slot;
+        if (inside) {
 #pragma unroll
-        for (int n = 0; n < Sh::kDmas; ++n) {
-          const uint32_t c = chunk_of(keys, n);
-          const int32_t row = clamp_key(t0 + n * Sh::kRowsPerDma + row_l) - t0;
-          if (!PAD || c < (uint32_t)a.head_size * 2u)
-            dma_asm16(base, (uint32_t)row * (uint32_t)a.entry_stride + c, at + n * 1024);
+          for (int n = 0; n < Sh::kDmas; ++n)
+            if (!PAD || chunk_of(r, n) < (uint32_t)a.head_size * 2u) dma_asm16(base, off[r][n], to, n * 1024);
+        } else {
+#pragma unroll
+          for (int n = 0; n < Sh::kDmas; ++n) {
+            const int32_t row = clamp_key(t0 + n * Sh::kRowsPerDma + row_l) - t0;
+            const uint32_t c = chunk_of(r, n);
+            if (!PAD || c < (uint32_t)a.head_size * 2u)
+              dma_asm16(base, (uint32_t)row * (uint32_t)a.entry_stride + c, to, n * 1024);
+          }
         }
       }
     } else {
       const int32_t t = clamp_key(share_at(j) + (lane & 15));
       page = *(const __attribute__((address_space(3))) int32_t*)(
-          ids + (j % Sh::kIdSlots) * 256 + (lane & 15) * 4);
+          ids + (j % Sh::kIdSlots) * 64 + (lane & 15) * 4);
       const int64_t e = attn_clip_page(a, page) * a.page_stride +
                         (int64_t)(t - attn_page_of(a, t) * a.page_size) * a.entry_stride;
       const int32_t e_lo = (int32_t)e, e_hi = (int32_t)(e >> 32);
@@ -205,16 +220,12 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
         const int row = n * Sh::kRowsPerDma + row_l;
         const int64_t s = (int64_t)(((uint64_t)(uint32_t)__shfl(e_hi, row, 64) << 32) |
                                     (uint32_t)__shfl(e_lo, row, 64));
-        const uint32_t c = chunk_of(keys, n);
-        if (!PAD || c < (uint32_t)a.head_size * 2u) dma_asm16(cache + s + c, at + n * 1024);
+#pragma unroll
+        for (int r = 0; r < ROLES; ++r)
+          if (!PAD || off[r][n] < (uint32_t)a.head_size * 2u)
+            dma_asm16(src[r] + s + off[r][n], lds_addr(dst[r]) + slot, n * 1024);
       }
     }
-  };
-  auto load_k = [&](int32_t j, int32_t page) {
-    if (brings_k) load_share(j, page, kc, true, klds + (uint32_t)j % Sh::kKeySteps * Sh::kStepBytes);
-  };
-  auto load_v = [&](int32_t j, int32_t page) {
-    if (brings_v) load_share(j, page, vc, false, vlds + (uint32_t)j % Sh::kValueSteps * Sh::kStepBytes);
   };
 
   // ---- operand reads
@@ -282,30 +293,32 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
   auto body = [&](int32_t u, auto sub, Scores& cur, Scores& next, auto more) {
     constexpr bool MORE = decltype(more)::value;
     constexpr int SUB = decltype(sub)::value;  // u & 1
-    const uint32_t v_at = (uint32_t)u / 2 % Sh::kValueSteps * Sh::kStepBytes;
-    const uint32_t k_at = ((uint32_t)u + 1) / 2 % Sh::kKeySteps * Sh::kStepBytes;
+    const uint32_t v_at = (uint32_t)u / 2 % Sh::kSteps * Sh::kStepBytes;
+    const uint32_t k_at = ((uint32_t)u + 1) / 2 % Sh::kSteps * Sh::kStepBytes;
+    constexpr int PV = 2 * DTILES;      // operands of the output's products
     constexpr int PER = QT * 16 / KSTEPS;  // probabilities per operand of the next scores
-    constexpr int PV = 2 * DTILES;         // operands of the output's products
-    constexpr int PERM = QT * 16 / PV;     // scores that enter the maximum per such operand
-    u32x4 p[QT][2], kf[3], vf[3];
+    constexpr int PERM = QT * 16 / PV;  // scores that enter the maximum per operand
+    u32x4 p[QT][2], kf[AHEAD + 1], vf[AHEAD + 1];
     if constexpr (MORE) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) next.s[qt][i] = 0.f;
-      kf[0] = read_k(k_at, SUB ^ 1, 0);
-      kf[1] = read_k(k_at, SUB ^ 1, 1);
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) kf[n] = read_k(k_at, SUB ^ 1, n);
     }
 #pragma unroll
     for (int n = 0; n < KSTEPS; ++n) {
       if constexpr (MORE) {
-        if (n + 2 < KSTEPS) kf[(n + 2) % 3] = read_k(k_at, SUB ^ 1, n + 2);
+        if (n + AHEAD < KSTEPS) kf[(n + AHEAD) % (AHEAD + 1)] = read_k(k_at, SUB ^ 1, n + AHEAD);
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt)
-          next.s[qt] = mfma32x16<DT>(kf[n % 3], q[qt][n], next.s[qt]);
+          next.s[qt] = mfma32x16<DT>(kf[n % (AHEAD + 1)], q[qt][n], next.s[qt]);
       }
-      if (n == KSTEPS - 2) vf[0] = read_v(v_at, SUB, 0, 0);
-      if (n == KSTEPS - 1) vf[1] = read_v(v_at, SUB, 0, 1);
+      if (n >= KSTEPS - AHEAD) {
+        const int i = n - (KSTEPS - AHEAD);
+        vf[i] = read_v(v_at, SUB, i / DTILES, i % DTILES);
+      }
 #pragma unroll
       for (int e = n * PER; e < (n + 1) * PER; e += 2) {
         const int qt = e / 16, i = e % 16;
@@ -324,10 +337,11 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
     for (int qt = 0; qt < QT; ++qt) top[qt] = -INFINITY;
 #pragma unroll
     for (int n = 0; n < PV; ++n) {
-      if (n + 2 < PV) vf[(n + 2) % 3] = read_v(v_at, SUB, (n + 2) / DTILES, (n + 2) % DTILES);
+      if (n + AHEAD < PV)
+        vf[(n + AHEAD) % (AHEAD + 1)] = read_v(v_at, SUB, (n + AHEAD) / DTILES, (n + AHEAD) % DTILES);
       const int ks = n / DTILES, dt = n % DTILES;
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt) o[dt][qt] = mfma32x16<DT>(vf[n % 3], p[qt][ks], o[dt][qt]);
+      for (int qt = 0; qt < QT; ++qt) o[dt][qt] = mfma32x16<DT>(vf[n % (AHEAD + 1)], p[qt][ks], o[dt][qt]);
       if constexpr (MORE) {
 #pragma unroll
         for (int e = n * PERM; e < (n + 1) * PERM; e += 2) {
@@ -346,18 +360,11 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
       for (int i = 0; i < 6; ++i) load_ids(i);
       wait_vmcnt<0>();
     }
-    // pages of the steps whose keys, resp. values, are asked for next
-    int32_t page_v = share_page(2), page_k = share_page(3);
-    {
-      const int32_t p0 = share_page(0), p1 = share_page(1);
-      load_k(0, p0);
-      load_k(1, p1);
-      load_v(0, p0);
-      load_k(2, page_v);
-      load_v(1, p1);
-    }
-    // keys of step 0 (8 waves: steps 0 and 1 are all that a wave has asked for besides keys 2)
-    if constexpr (WAVES == 4) wait_vmcnt<4 * Sh::kDmas>(); else wait_vmcnt<Sh::kDmas>();
+    int32_t page = share_page(3);  // of the step that is asked for next
+    load_step(0, share_page(0));
+    load_step(1, share_page(1));
+    load_step(2, share_page(2));
+    wait_vmcnt<2 * ROLES * Sh::kDmas>();  // step 0
     wave_barrier();
     Scores s0, s1;
     {
@@ -381,17 +388,15 @@ void paged_attn_tile_kernel(PagedAttnArgs a) {
       }
       raise(top);
     }
-    // Step j: keys j + 1 and values j have landed once only what step j - 1 asked for is missing
-    // (before the first: keys 2 and values 1).
+    // Step j needs keys up to j + 1 and values j: all but what step j - 1 has asked for (before the
+    // first: step 2).
     int32_t j = 0;
-    if constexpr (WAVES == 4) wait_vmcnt<2 * Sh::kDmas>(); else wait_vmcnt<0>();
+    wait_vmcnt<ROLES * Sh::kDmas>();
     while (j + 1 < steps) {
       wave_barrier();
-      load_k(j + 3, page_k);
-      load_v(j + 2, page_v);
+      load_step(j + 3, page);
       load_ids(j + 6);
-      page_v = page_k;
-      page_k = share_page(j + 4);
+      page = share_page(j + 4);
       body(2 * j, std::integral_constant<int, 0>{}, s0, s1, std::true_type{});
       body(2 * j + 1, std::integral_constant<int, 1>{}, s1, s0, std::true_type{});
       wait_vmcnt<kOps>();

@@ -41,7 +41,7 @@ struct PagedAttnArgs {
   int32_t* part_map;      // [seqs + 1] first item, then [seqs] parts per tile
   int64_t q_stride, out_stride;           // elements
   int64_t page_stride, entry_stride;      // bytes
-  uint64_t page_magic;    // ceil(2^page_shift / page_size): division of positions by page_size
+  uint32_t page_magic;    // ceil(2^page_shift / page_size): division of positions by page_size
   uint32_t page_shift;
   int32_t seqs, tokens, heads, kv_heads, group, head_size;
   int32_t page_size, num_pages, num_indices;
@@ -82,7 +82,7 @@ SK_DEV void attn_span(const PagedAttnArgs& a, const AttnSeq& x, int32_t j, int32
 
 // Position -> index of its page in the request's part of kv_indices.
 SK_DEV int32_t attn_page_of(const PagedAttnArgs& a, int32_t pos) {
-  return (int32_t)(((uint64_t)(uint32_t)pos * a.page_magic) >> a.page_shift);
+  return (int32_t)(((uint64_t)(uint32_t)pos * (uint64_t)a.page_magic) >> a.page_shift);
 }
 // A page number outside the cache is never followed: the last page stands in for it.
 SK_DEV int32_t attn_clip_page(const PagedAttnArgs& a, int32_t page) {
@@ -265,14 +265,15 @@ SK_DEV u32x2 lds_read_tr_b64(const lds_char* p) {
 // dma_to_lds() as instructions that the compiler does not look into: it places no waits for them, so
 // every read of what they bring stands behind a counted wait_vmcnt() (and a barrier, where another
 // wave loaded it).  No register is written but M0, which nothing else in those kernels uses.
-SK_DEV void dma_asm16(const void* src, lds_char* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_addr(base)), "v"(src)
-               : "memory");
+// `to` is the LDS address of the first lane, less `plus` (a constant).
+SK_DEV void dma_asm16(const void* src, uint32_t to, int plus) {
+  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src), "n"(plus)
+               : "memory", "scc");
 }
-SK_DEV void dma_asm16(const char* uniform_base, uint32_t off, lds_char* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_addr(base)), "v"(off),
-               "s"(uniform_base)
-               : "memory");
+SK_DEV void dma_asm16(const char* uniform_base, uint32_t off, uint32_t to, int plus) {
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off),
+               "s"(uniform_base), "n"(plus)
+               : "memory", "scc");
 }
 SK_DEV void dma_asm4(const void* src, lds_char* base) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr(base)), "v"(src)
