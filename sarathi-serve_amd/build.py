@@ -25,7 +25,9 @@ HIP_SOURCES = ["rms_norm.hip", "gated_act.hip", "rope.hip", "moe_topk.hip", "moe
                "moe_gemm.hip", "moe_gemm_wide.hip", "moe_sum.hip", "kv_cache.hip",
                "moe_fused_routing.hip", "stream_copy.hip", "moe_balance.hip", "moe_gemm_f32.hip",
                "moe_gemm_rider.hip", "kv_metadata.hip", "paged_attention.hip",
-               "paged_attention_tiles.hip", "merge_states.hip"]
+               "paged_attention_few.hip", "paged_attention_mixed_bf16_64.hip",
+               "paged_attention_mixed_bf16_128.hip", "paged_attention_mixed_f16_64.hip",
+               "paged_attention_mixed_f16_128.hip", "merge_states.hip"]
 CXX_SOURCES = ["abi_misc.cpp"]
 
 ABI_LIB = os.path.join(LIB_DIR, "libsarathi_ops_hip.so")
@@ -43,9 +45,10 @@ HIP_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=16",
     "-Wall", "-Wno-unused-command-line-argument",
 ]
-# Per source: the tile kernel of the attention wants the results of its matrix instructions in
-# registers that the vector unit can read (its softmax works on them).
-SOURCE_FLAGS = {"paged_attention_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# Per source: the matrix-core attention kernels want the results of their matrix instructions in
+# registers that the vector unit can read (the softmax works on them).
+SOURCE_FLAGS = {src: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for src in HIP_SOURCES
+                if src.startswith("paged_attention_")}
 # extra hipcc flags for tuning builds, e.g. -DSARATHI_KV_STORE_POLICY=18
 HIP_FLAGS += os.environ.get("SARATHI_HIPCC_EXTRA_FLAGS", "").split()
 

@@ -3,11 +3,12 @@
 // (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:169-209, 262-304): one entry
 // for chunks of new tokens and for single decode tokens alike.
 //
-// This file holds the kernel for few rows (decode steps), the plain kernel for any head size and
-// alignment, the kernel that joins the parts of a cut context, and the entry point that chooses.
+// This file holds the entry point, the plan of a launch, the plain kernel for any head size and
+// alignment and the kernel that joins the parts of a cut context; the matrix-core kernels are in
+// paged_attention_few.hip and paged_attention_mixed_*.hip.
 #include "launch.h"
 #include "paged_attn.h"
-#include "paged_attn_tiles.h"
+#include "paged_attn_launch.h"
 
 namespace sarathi_hip {
 
@@ -80,396 +81,206 @@ __global__ __launch_bounds__(64) void paged_attn_plain_kernel(PagedAttnArgs a) {
   if (a.lse && lane == 0) a.lse[(int64_t)tok * a.heads + head] = attn_lse(m, l);
 }
 
-// ---- few rows: decode steps --------------------------------------------------------------------
-//
-// Bound by the bytes of the keys and values.  A workgroup is four waves that share one tile of
-// 16 * RT rows and stream its keys 16 at a time, each wave through a ring in LDS of its own
-// (kFewStages blocks of 16 keys and values, filled by loads that write LDS directly), so that no
-// wave waits for another before the end: there the four states are joined through LDS.
-//   scores  S^T = K Q^T: keys as rows, the tile's rows as columns, so a row's softmax stays inside
-//           four lanes (lane & 15 names the row), and the probabilities come out of the product in
-//           the very layout in which
-//   output  O^T += V^T P^T takes them: no exchange between lanes, V is transposed by the LDS read.
-// Chunks of 16 bytes are stored swizzled, K by XOR with the row so that sixteen rows' same chunk
-// lie in different banks, V by XOR of chunk pairs so that eight rows' same sixteen elements do.
-// Probabilities are rounded to the cache's type for the product (at most half a step each, of
-// values up to 1); maximum, sum and output stay in 32 bits.
-template <int DP> struct FewShape {
-  static constexpr int kRowBytes = DP * 2;
-  static constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
-  static constexpr int kRowsPerDma = 64 / kChunks;  // rows one load instruction moves
-  static constexpr int kDmas = 16 / kRowsPerDma;    // per block of 16 keys (and as many for values)
-  static constexpr int kStages = DP >= 256 ? 2 : DP == 128 ? 2 : 4;
-  static constexpr int kBlockBytes = 16 * kRowBytes;
-  static constexpr int kIdSlots = 2 * kStages;
-  static constexpr int kWaveBytes = kStages * 2 * kBlockBytes + kIdSlots * 256;
-  SK_DEV static int swz_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
-  SK_DEV static int swz_v(int row) { return DP == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; }
-};
-
-template <int DT, int DP, int RT, bool PAD>
-__global__ __launch_bounds__(256) void paged_attn_few_kernel(PagedAttnArgs a) {
-  using Sh = FewShape<DP>;
-  constexpr int ROWS = 16 * RT, S = Sh::kStages, KSTEPS = DP / 32, DTILES = DP / 16;
-  constexpr int kOps = 2 * Sh::kDmas + 1;  // loads a block takes: keys, values, page numbers
-  extern __shared__ u32x4 few_lds[];
-  const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
-  const AttnItem it = attn_find_item<ROWS, 4>(a, blockIdx.x / (uint32_t)a.kv_heads,
-                                              a.part_map != nullptr && blockIdx.x == 0);
-  if (it.r < 0) return;
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const AttnSeq x = attn_seq(a, it.r);
-  const int32_t rows_all = x.n * a.group, row0 = it.tile * ROWS;
-  const int32_t rows = rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
-
-  // this lane's rows (one per row tile): query operand, span of keys
-  u32x4 q[RT][KSTEPS];
-  int32_t lo[RT], hi[RT], tok[RT], head[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int32_t i = rt * 16 + col;
-    const int32_t p = row0 + (i < rows ? i : rows - 1);
-    const int32_t j = p / a.group;
-    tok[rt] = x.q0 + j;
-    head[rt] = (int32_t)h * a.group + (p - j * a.group);
-    attn_span(a, x, j, lo[rt], hi[rt]);
-    const char* src = reinterpret_cast<const char*>(a.q) +
-                      ((int64_t)tok[rt] * a.q_stride + (int64_t)head[rt] * a.head_size) * 2;
-#pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
-      const int d = k * 32 + g * 8;
-      q[rt][k] = d < a.head_size ? *reinterpret_cast<const u32x4*>(src + d * 2) : u32x4{0, 0, 0, 0};
-    }
-  }
-  // some row sees [span_lo, span_hi), every row [full_lo, full_hi)
-  int32_t span_lo, span_hi, full_lo, full_hi;
-  attn_span(a, x, row0 / a.group, span_lo, full_hi);
-  attn_span(a, x, (row0 + rows - 1) / a.group, full_lo, span_hi);
-  full_lo = __builtin_amdgcn_readfirstlane(full_lo);
-  full_hi = __builtin_amdgcn_readfirstlane(full_hi);
-  const int32_t begin = __builtin_amdgcn_readfirstlane(
-      it.parts > 1 ? (int32_t)min((int64_t)span_hi, span_lo + (int64_t)it.part * it.part_len) : span_lo);
-  const int32_t end = __builtin_amdgcn_readfirstlane(
-      it.parts > 1 ? (int32_t)min((int64_t)span_hi, (int64_t)begin + it.part_len) : span_hi);
-
-  float m[RT], l[RT];
-  f32x4 o[RT][DTILES];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
-    l[rt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < DTILES; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-
-  lds_char* const base = (lds_char*)few_lds + wave * Sh::kWaveBytes;
-  lds_char* const ids = base + S * 2 * Sh::kBlockBytes;
-  if constexpr (PAD) {  // chunks beyond the head are never loaded: they stay zero
-    for (int i = lane * 16; i < S * 2 * Sh::kBlockBytes; i += 1024)
-      *(__attribute__((address_space(3))) u32x4*)(base + i) = u32x4{0, 0, 0, 0};
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
-  // blocks of 16 keys are dealt to the waves in turn
-  const int32_t total = end - begin;
-  const int32_t nb = total > wave * 16 ? (total - wave * 16 + 63) / 64 : 0;
-  auto key_of = [&](int32_t b, int row) {  // past the end: the last key again
-    const int32_t t = begin + (b * 4 + wave) * 16 + row;
-    return t < end ? t : end - 1;
-  };
-  auto load_ids = [&](int32_t b) {
-    const int32_t* src = a.kv_indices + x.kv0 + attn_page_of(a, key_of(b, col));
-    dma_to_lds<4>(src, ids + (b % Sh::kIdSlots) * 256);  // four copies, no lane off
-  };
-  const char* const kc = reinterpret_cast<const char*>(a.k_cache) + (int64_t)h * a.head_size * 2;
-  const char* const vc = reinterpret_cast<const char*>(a.v_cache) + (int64_t)h * a.head_size * 2;
-  auto load_block = [&](int32_t b) {
-    const int32_t t = key_of(b, col);
-    const int32_t pg = attn_page_of(a, t);
-    const int32_t page = attn_clip_page(
-        a, *(const __attribute__((address_space(3))) int32_t*)(ids + (b % Sh::kIdSlots) * 256 + col * 4));
-    const int64_t off = page * a.page_stride + (int64_t)(t - pg * a.page_size) * a.entry_stride;
-    const int32_t off_lo = (int32_t)off, off_hi = (int32_t)(off >> 32);
-    lds_char* const dst = base + (b % S) * 2 * Sh::kBlockBytes;
-#pragma unroll
-    for (int n = 0; n < Sh::kDmas; ++n) {
-      const int row = n * Sh::kRowsPerDma + lane / Sh::kChunks, pos = lane % Sh::kChunks;
-      const int64_t e = (int64_t)(((uint64_t)(uint32_t)__shfl(off_hi, row, 64) << 32) |
-                                  (uint32_t)__shfl(off_lo, row, 64));
-      const int ck = pos ^ Sh::swz_k(row), cv = pos ^ Sh::swz_v(row);
-      if (!PAD || ck * 8 < a.head_size) dma_to_lds<16>(kc + e + ck * 16, dst + n * 1024);
-      if (!PAD || cv * 8 < a.head_size)
-        dma_to_lds<16>(vc + e + cv * 16, dst + Sh::kBlockBytes + n * 1024);
-    }
-  };
-
-  if (nb > 0) {
-#pragma unroll
-    for (int i = 0; i < S; ++i) load_ids(i);
-    wait_vmcnt<0>();
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      load_block(i);
-      load_ids(S + i);
-    }
-  }
-  for (int32_t b = 0; b < nb; ++b) {
-    // everything up to this block's values and the page numbers of block b + S
-    wait_vmcnt<(S - 1) * kOps>();
-    const lds_char* const kb = base + (b % S) * 2 * Sh::kBlockBytes;
-    const lds_char* const vb = kb + Sh::kBlockBytes;
-    const int32_t t0 = begin + (b * 4 + wave) * 16;
-    f32x4 s[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) s[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
-      const u32x4 kk = *(const __attribute__((address_space(3))) u32x4*)(
-          kb + col * Sh::kRowBytes + (((k * 4 + g) ^ Sh::swz_k(col)) * 16));
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt] = mfma16x32<DT>(kk, q[rt][k], s[rt]);
-    }
-    const bool whole = t0 >= full_lo && t0 + 16 <= full_hi && t0 + 16 <= end;
-    u32x2 p[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float z[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) z[j] = s[rt][j] * a.scale_log2;
-      if (!whole) {
-        const int32_t top = hi[rt] < end ? hi[rt] : end;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int32_t t = t0 + g * 4 + j;
-          z[j] = t >= lo[rt] && t < top ? z[j] : -INFINITY;
-        }
-      }
-      const float top = fmaxf(m[rt], group_max(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]))));
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float keep = __builtin_amdgcn_exp2f(m[rt] - ref);
-      m[rt] = top;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) z[j] = __builtin_amdgcn_exp2f(z[j] - ref);
-      l[rt] = l[rt] * keep + ((z[0] + z[1]) + (z[2] + z[3]));
-      p[rt] = u32x2{pack2<DT>(z[0], z[1]), pack2<DT>(z[2], z[3])};
-#pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt) o[rt][dt] *= keep;
-    }
-    const int vrow = g * 4 + (col >> 2);
-    const uint32_t vaddr = lds_addr(vb + vrow * Sh::kRowBytes + (col & 1) * 8);
-#pragma unroll
-    for (int d0 = 0; d0 < DTILES; d0 += 4) {
-      uint32_t at[4];
-      u32x2 vv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        at[i] = vaddr + ((((d0 + i) * 2 + ((col >> 1) & 1)) ^ Sh::swz_v(vrow)) * 16);
-      lds_read_tr4(at, vv);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][d0 + i] = mfma16x16<DT>(vv[i], p[rt], o[rt][d0 + i]);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the block is read: its place can be filled
-    load_block(b + S);
-    load_ids(b + 2 * S);
-  }
-  wait_vmcnt<0>();
-  __syncthreads();
-
-  // join the four waves: 2 and 3 hand over to 0 and 1, then 1 to 0
-  typedef __attribute__((address_space(3))) float lds_float;
-  constexpr int kState = 64 * (2 + DTILES * 4) * RT;  // floats a wave hands over
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) l[rt] = group_sum(l[rt]);
-#pragma unroll
-  for (int step = 2; step > 0; step >>= 1) {
-    lds_float* const box = (lds_float*)few_lds + (wave & (step - 1)) * kState;
-    if (wave >= step && wave < 2 * step) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        lds_float* const b = box + rt * 64 * (2 + DTILES * 4);
-        b[lane] = m[rt];
-        b[64 + lane] = l[rt];
-#pragma unroll
-        for (int dt = 0; dt < DTILES; ++dt)
-          *(__attribute__((address_space(3))) f32x4*)(b + 128 + dt * 256 + lane * 4) = o[rt][dt];
-      }
-    }
-    __syncthreads();
-    if (wave < step) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        lds_float* const b = box + rt * 64 * (2 + DTILES * 4);
-        const float m2 = b[lane], l2 = b[64 + lane];
-        const float top = fmaxf(m[rt], m2), ref = top == -INFINITY ? 0.f : top;
-        const float w1 = __builtin_amdgcn_exp2f(m[rt] - ref), w2 = __builtin_amdgcn_exp2f(m2 - ref);
-        m[rt] = top;
-        l[rt] = l[rt] * w1 + l2 * w2;
-#pragma unroll
-        for (int dt = 0; dt < DTILES; ++dt)
-          o[rt][dt] = o[rt][dt] * w1 +
-                      *(__attribute__((address_space(3))) f32x4*)(b + 128 + dt * 256 + lane * 4) * w2;
-      }
-    }
-    __syncthreads();
-  }
-  if (wave != 0) return;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    if (rt * 16 + col >= rows) continue;
-    if (it.parts > 1) {
-      const int64_t slot = ((int64_t)it.index * a.kv_heads + h) * ROWS + rt * 16 + col;
-      if (g == 0) {
-        a.part_ml[slot * 2] = m[rt];
-        a.part_ml[slot * 2 + 1] = l[rt];
-      }
-#pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt)
-        if (dt * 16 + g * 4 < a.head_size)
-          *reinterpret_cast<f32x4*>(a.part_o + slot * a.head_size + dt * 16 + g * 4) = o[rt][dt];
-    } else {
-      const float inv = l[rt] == 0.f ? 0.f : 1.f / l[rt];
-      char* const dst = reinterpret_cast<char*>(a.out) +
-                        ((int64_t)tok[rt] * a.out_stride + (int64_t)head[rt] * a.head_size) * 2;
-#pragma unroll
-      for (int dt = 0; dt < DTILES; ++dt)
-        if (dt * 16 + g * 4 < a.head_size)
-          *reinterpret_cast<u32x2*>(dst + (dt * 16 + g * 4) * 2) =
-              u32x2{pack2<DT>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
-                    pack2<DT>(o[rt][dt][2] * inv, o[rt][dt][3] * inv)};
-      if (a.lse && g == 0) a.lse[(int64_t)tok[rt] * a.heads + head[rt]] = attn_lse(m[rt], l[rt]);
-    }
-  }
-}
-
 // ---- joins the parts of cut contexts -------------------------------------------------------------
 //
-// One wave per token and query head; parts whose sum is zero have no output.  Parts are added in
-// their order, so results do not depend on which workgroup ran when.
-template <int DT, int VALS>  // VALS elements of the head per lane
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a, int32_t rows_per_tile) {
-  const int lane = threadIdx.x & 63;
-  const int32_t head = (int32_t)blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int32_t tok = (int32_t)blockIdx.x;
-  if (head >= a.heads) return;
-  if (tok >= clamp_i32(a.qo_indptr[a.seqs], 0, a.tokens) || tok < a.qo_indptr[0]) return;
-  int32_t r = 0, hi_r = a.seqs;
-  while (hi_r - r > 1) {
-    const int32_t mid = (r + hi_r) >> 1;
-    if (a.qo_indptr[mid] <= tok) r = mid; else hi_r = mid;
-  }
-  const int32_t parts = a.part_map[a.seqs + r];
-  if (parts <= 1) return;
-  const AttnSeq x = attn_seq(a, r);
-  if (tok < x.q0 || tok >= x.q0 + x.n) return;
-  const int32_t h = head / a.group;
-  const int32_t row = (tok - x.q0) * a.group + (head - h * a.group);
-  const int32_t tile = row / rows_per_tile, in_tile = row - tile * rows_per_tile;
-  const int64_t item0 = (int64_t)a.part_map[r] + (int64_t)tile * parts;
-  auto slot_of = [&](int32_t p) {
-    return ((item0 + p) * a.kv_heads + h) * rows_per_tile + in_tile;
-  };
-  float m = -INFINITY;
-  for (int32_t p = lane; p < parts; p += 64) {
-    const int64_t s = slot_of(p);
-    if (a.part_ml[s * 2 + 1] != 0.f) m = fmaxf(m, a.part_ml[s * 2]);
-  }
-  m = wave64_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[VALS] = {};
-  const int d0 = lane * VALS;
-  const bool on = d0 < a.head_size;
-#pragma unroll 4
-  for (int32_t p = 0; p < parts; ++p) {
-    const int64_t s = slot_of(p);
-    const float pl = a.part_ml[s * 2 + 1];
-    const float w = pl != 0.f ? __builtin_amdgcn_exp2f(a.part_ml[s * 2] - ref) : 0.f;
-    l += pl * w;
-    if (on && pl != 0.f) {
-#pragma unroll
-      for (int i = 0; i < VALS; ++i) o[i] = fmaf(a.part_o[s * a.head_size + d0 + i], w, o[i]);
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (on) {
-    const int64_t base = (int64_t)tok * a.out_stride + (int64_t)head * a.head_size + d0;
-#pragma unroll
-    for (int i = 0; i < VALS; ++i) store_elem<DT>(a.out, base + i, o[i] * inv);
-  }
-  if (a.lse && lane == 0) a.lse[(int64_t)tok * a.heads + head] = attn_lse(m, l);
-}
+// WPT waves per token and four query heads of a key head: sixteen where there are few tokens (a
+// workgroup of their own), else one (four tokens in a workgroup).  Half-waves of 32 lanes share the
+// rows and their parts: with few rows several take turns at one row's parts, and each has eight of them on
+// their way at once, so that the time hardly grows with the parts.  A part whose sum is zero has no
+// output.  Parts are added in a fixed order: results do not depend on which workgroup ran when.
+// Nothing to join (the attention kernel leaves word) costs a launch and one load.
+constexpr int kJoinRows = 4;
 
-template <int DT, int DP, int RT>
-static int launch_few(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
-  constexpr int ring = 4 * FewShape<DP>::kWaveBytes;
-  constexpr int join = 2 * 64 * (2 + DP / 16 * 4) * RT * 4;
-  constexpr int bytes = ring > join ? ring : join;
-  const dim3 grid((unsigned)groups), block(256);
-  if (a.head_size == DP) {
-    if (!allow_lds<paged_attn_few_kernel<DT, DP, RT, false>>(bytes)) return SARATHI_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_attn_few_kernel<DT, DP, RT, false>), grid, block, bytes, st, a);
+template <int DT, int VALS, int WPT>  // VALS elements of the head per lane
+__global__ __launch_bounds__(WPT == 1 ? 256 : WPT * 64) void paged_attn_join_kernel(PagedAttnArgs a) {
+  constexpr int U = 2 * WPT;  // half-waves of a token
+  typedef float vals_t __attribute__((ext_vector_type(VALS)));
+  __shared__ float box[WPT == 1 ? 1 : WPT][32 * VALS + 2];
+  const int lane = threadIdx.x & 63, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int unit = WPT == 1 ? lane >> 5 : (int)threadIdx.x >> 5;
+  const int32_t tok = (int32_t)blockIdx.x * (WPT == 1 ? 4 : 1) + (WPT == 1 ? wave : 0);
+  const int32_t quads = (a.group + kJoinRows - 1) / kJoinRows;
+  const int32_t h = (int32_t)blockIdx.y / quads, g_first = ((int32_t)blockIdx.y - h * quads) * kJoinRows;
+  const int32_t g_end = g_first + kJoinRows < a.group ? g_first + kJoinRows : a.group;
+  // one trip to memory for everything, where 64 lanes hold all requests
+  const bool small = a.seqs < 64;
+  const int32_t any = a.part_map[2 * a.seqs];
+  const int32_t li = lane <= a.seqs ? lane : a.seqs, lr = lane < a.seqs ? lane : a.seqs - 1;
+  int32_t qo_l = 0, row_l = 0, parts_l = 0;
+  if (small) {
+    qo_l = a.qo_indptr[li];
+    row_l = a.part_map[lr];
+    parts_l = a.part_map[a.seqs + lr];
+  }
+  if (any == 0 || tok >= a.tokens) return;
+  // request of the token, the last whose first token is not past it
+  int32_t r = 0, parts, first_row, q0, n;
+  if (small) {
+    const int cnt = __popcll(__builtin_amdgcn_ballot_w64(lane < a.seqs && qo_l <= tok));
+    if (cnt == 0) return;  // before the first request
+    r = cnt - 1;
+    parts = __builtin_amdgcn_readlane(parts_l, r);
+    first_row = __builtin_amdgcn_readlane(row_l, r);
+    q0 = clamp_i32(__builtin_amdgcn_readlane(qo_l, r), 0, a.tokens);
+    n = clamp_i32(__builtin_amdgcn_readlane(qo_l, r + 1), q0, a.tokens) - q0;
   } else {
-    if (!allow_lds<paged_attn_few_kernel<DT, DP, RT, true>>(bytes)) return SARATHI_ERR_LAUNCH;
-    hipLaunchKernelGGL((paged_attn_few_kernel<DT, DP, RT, true>), grid, block, bytes, st, a);
+    int32_t width = a.seqs;
+    while (true) {  // 64 candidates at a time
+      const int32_t step = (width + 63) / 64;
+      const bool ok = lane * step < width && a.qo_indptr[r + lane * step] <= tok;
+      const int cnt = __popcll(__builtin_amdgcn_ballot_w64(ok));
+      if (cnt == 0) return;
+      r += (cnt - 1) * step;
+      if (step == 1) break;
+      width = width - (cnt - 1) * step < step ? width - (cnt - 1) * step : step;
+    }
+    r = __builtin_amdgcn_readfirstlane(r);
+    parts = a.part_map[a.seqs + r];
+    first_row = a.part_map[r];
+    q0 = clamp_i32(a.qo_indptr[r], 0, a.tokens);
+    n = clamp_i32(a.qo_indptr[r + 1], q0, a.tokens) - q0;
   }
-  return launch_status();
-}
-template <int DT, int DP>
-static int launch_few_rows(const PagedAttnArgs& a, int row_tiles, int64_t groups, hipStream_t st) {
-  if (row_tiles == 1) return launch_few<DT, DP, 1>(a, groups, st);
-  if constexpr (DP <= 128)
-    if (row_tiles == 4) return launch_few<DT, DP, 4>(a, groups, st);
-  return launch_few<DT, DP, 2>(a, groups, st);
-}
-template <int DT>
-static int launch_few_heads(const PagedAttnArgs& a, int row_tiles, int64_t groups, hipStream_t st) {
-  if (a.head_size <= 64) return launch_few_rows<DT, 64>(a, row_tiles, groups, st);
-  if (a.head_size <= 128) return launch_few_rows<DT, 128>(a, row_tiles, groups, st);
-  return launch_few_rows<DT, 256>(a, row_tiles, groups, st);
+  if (parts <= 1 || tok < q0 || tok >= q0 + n) return;
+  const int64_t rows_all = (int64_t)n * a.group;
+  const bool tiled = a.few.rows_log2 < 0 || (a.tile.rows_log2 >= 0 && rows_all > a.few.max_rows);
+  const int32_t lg = tiled ? a.tile.rows_log2 : a.few.rows_log2;
+  int share = U;  // half-waves per row
+  while (share > 1 && U / share < g_end - g_first) share >>= 1;
+  const int rows_at_once = U / share;
+  const int d0 = l32 * VALS;
+  const bool on = d0 < a.head_size;
+  for (int32_t g0 = g_first; g0 < g_end; g0 += rows_at_once) {
+    const int32_t gq = g0 + unit / share;
+    const bool live = gq < g_end;
+    const int32_t row = (tok - q0) * a.group + (live ? gq : g_first);
+    const int32_t tile = row >> lg, in_tile = row & ((1 << lg) - 1);
+    const int64_t row0 = first_row + ((int64_t)(tile * parts * a.kv_heads + h) << lg) + in_tile;
+    const int64_t per_part = (int64_t)a.kv_heads << lg;
+    float ref = kRefStart, l = 0.f;
+    vals_t o = 0.f;
+    for (int32_t p0 = unit % share; p0 < parts; p0 += 8 * share) {
+      f32x2 ml[8];
+      vals_t po[8];
+      float pr[8], pl[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int32_t p = p0 + i * share;
+        const int64_t at = row0 + (p < parts ? p : parts - 1) * per_part;
+        ml[i] = *reinterpret_cast<const f32x2*>(a.part_ml + at * 2);
+        // heads are multiples of 8 elements: whole vectors; lanes past the head read its first
+        po[i] = *reinterpret_cast<const vals_t*>(a.part_o + at * a.head_size + (on ? d0 : 0));
+      }
+      __builtin_amdgcn_sched_barrier(0);  // every load is issued before anything waits
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        pr[i] = ml[i].x;
+        pl[i] = p0 + i * share < parts ? ml[i].y : 0.f;
+      }
+      float top = ref;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = pl[i] != 0.f ? fmaxf(top, pr[i]) : top;
+      const float keep = __builtin_amdgcn_exp2f(ref - top);
+      ref = top;
+      l *= keep;
+      o *= keep;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = pl[i] != 0.f ? __builtin_amdgcn_exp2f(pr[i] - ref) : 0.f;
+        l += pl[i] * w;
+#pragma unroll
+        for (int v = 0; v < VALS; ++v) {
+          const float x = po[i][v];
+          o[v] = pl[i] != 0.f ? fmaf(x, w, o[v]) : o[v];
+        }
+      }
+    }
+    if (share > 1) {  // the two halves of a wave have the same row
+      const float ref2 = __shfl_xor(ref, 32, 64), l2 = __shfl_xor(l, 32, 64);
+      const float top = fmaxf(ref, ref2);
+      const float w1 = __builtin_amdgcn_exp2f(ref - top), w2 = __builtin_amdgcn_exp2f(ref2 - top);
+      l = l * w1 + l2 * w2;
+#pragma unroll
+      for (int v = 0; v < VALS; ++v) {
+        const float x = o[v];
+        o[v] = x * w1 + __shfl_xor(x, 32, 64) * w2;
+      }
+      ref = top;
+    }
+    if constexpr (WPT > 1) {
+      if (share > 2) {  // uniform over the workgroup
+        __syncthreads();  // the last round's boxes are read
+        if (lane < 32) {
+          box[wave][32 * VALS] = ref;
+          box[wave][32 * VALS + 1] = l;
+#pragma unroll
+          for (int v = 0; v < VALS; ++v) box[wave][d0 + v] = o[v];
+        }
+        __syncthreads();
+        if (unit % share == 0) {
+          float top = kRefStart;
+          for (int s = 0; s < share / 2; ++s) top = fmaxf(top, box[wave + s][32 * VALS]);
+          l = 0.f;
+          o = 0.f;
+          for (int s = 0; s < share / 2; ++s) {
+            const float w = __builtin_amdgcn_exp2f(box[wave + s][32 * VALS] - top);
+            l += box[wave + s][32 * VALS + 1] * w;
+#pragma unroll
+            for (int v = 0; v < VALS; ++v) o[v] += box[wave + s][d0 + v] * w;
+          }
+          ref = top;
+        }
+      }
+    }
+    if (unit % share != 0 || !live) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int32_t head = h * a.group + gq;
+    if (on) {
+      const int64_t base = (int64_t)tok * a.out_stride + (int64_t)head * a.head_size + d0;
+#pragma unroll
+      for (int v = 0; v < VALS; v += 2) {
+        const float x = o[v], y = o[v + 1];
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(a.out) + (base + v) * 2) = pack2<DT>(x * inv, y * inv);
+      }
+    }
+    if (a.lse && l32 == 0) a.lse[(int64_t)tok * a.heads + head] = attn_lse(ref, l);
+  }
 }
 
-template <int DT>
-static int launch_join(const PagedAttnArgs& a, int rows_per_tile, hipStream_t st) {
-  const dim3 grid((unsigned)a.tokens, (unsigned)((a.heads + 3) / 4));
-  if (a.head_size <= 64)
-    hipLaunchKernelGGL((paged_attn_join_kernel<DT, 1>), grid, dim3(256), 0, st, a, rows_per_tile);
-  else if (a.head_size <= 128)
-    hipLaunchKernelGGL((paged_attn_join_kernel<DT, 2>), grid, dim3(256), 0, st, a, rows_per_tile);
+template <int DT, int VALS> static int launch_join_head(const PagedAttnArgs& a, hipStream_t st) {
+  // sixteen waves per token while that leaves the GPU room
+  const unsigned heads4 = (unsigned)(a.kv_heads * ((a.group + kJoinRows - 1) / kJoinRows));
+  if ((int64_t)a.tokens * heads4 <= 2 * compute_units())
+    hipLaunchKernelGGL((paged_attn_join_kernel<DT, VALS, 16>), dim3((unsigned)a.tokens, heads4),
+                       dim3(1024), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_attn_join_kernel<DT, 4>), grid, dim3(256), 0, st, a, rows_per_tile);
+    hipLaunchKernelGGL((paged_attn_join_kernel<DT, VALS, 1>), dim3((unsigned)((a.tokens + 3) / 4), heads4),
+                       dim3(256), 0, st, a);
   return launch_status();
+}
+template <int DT> static int launch_join(const PagedAttnArgs& a, hipStream_t st) {
+  if (a.head_size <= 64) return launch_join_head<DT, 2>(a, st);
+  if (a.head_size <= 128) return launch_join_head<DT, 4>(a, st);
+  return launch_join_head<DT, 8>(a, st);
 }
 
 // ---- what a call launches ------------------------------------------------------------------------
 
 // The requests of a batch fall into two classes by their rows (new tokens times query heads per key
-// head): few rows, and chunks, which take the tile kernel.  All sizes here are known on the host.
-struct AttnClass {
-  int rows;            // rows per tile, 0: the class is empty
-  int32_t min_rows, max_rows;
-  int64_t tiles;       // at most so many tiles per key head
-  int32_t target, min_part;
-  int64_t items;       // at most so many items per key head
-  int64_t map_bytes, ml_bytes, o_bytes;  // of the workspace
-  int64_t bytes() const { return map_bytes + ml_bytes + o_bytes; }
-};
+// head): few rows, and chunks, which are taken in large tiles.  All sizes here are known on the host.
 struct AttnPlan {
   AttnClass few, tile;
+  int waves;           // of a workgroup
+  int64_t items;       // at most so many work items per key head, with contexts cut and without
+  int64_t uncut_items;
+  int64_t map_bytes, ml_bytes, o_bytes;  // of the workspace; 0: nothing is cut
+  int64_t bytes() const { return map_bytes + ml_bytes + o_bytes; }
 };
 static int64_t round256(int64_t v) { return (v + 255) & ~(int64_t)255; }
-
-// Aims at `items` work items per key head, of at least min_part keys each.
-static void plan_parts(AttnClass& c, int64_t items, int32_t min_part, int64_t seqs,
-                       int64_t capacity, int kv_heads, int head_size) {
-  const int64_t most = c.tiles * (capacity / min_part);  // no sequence is longer than all pages
-  c.min_part = min_part;
-  c.target = (int32_t)(items < most ? items : most);
-  c.items = c.tiles + c.target;
-  if (c.target <= 0) return;
-  c.map_bytes = round256((2 * seqs + 1) * 4);
-  c.ml_bytes = round256(c.items * kv_heads * c.rows * 8);
-  c.o_bytes = round256(c.items * kv_heads * c.rows * head_size * 4);
+static int log2_of(int v) {
+  int n = 0;
+  while ((1 << n) < v) ++n;
+  return n;
 }
 
 static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, int heads,
@@ -478,62 +289,80 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   const int group = heads / kv_heads;
   const int64_t longest = max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens;
   const int64_t most_rows = longest * group, all_rows = tokens * group;
-  const int64_t capacity = indices * page_size;
-  const int units = compute_units();
+  const int64_t capacity = indices * page_size;  // no sequence has more keys
+  const int64_t units = compute_units();
   const int few_limit = head_size > 128 ? 32 : 64;
-  AttnClass& f = p.few;
-  AttnClass& t = p.tile;
-  f.min_rows = 1;
+  int64_t few_tiles = 0, chunk_tiles = 0, few_target = 0, chunk_target = 0;
+  p.few.fill = 2 * units / kv_heads > 0 ? (int32_t)(2 * units / kv_heads) : 1;
+  p.tile.fill = units / kv_heads > 0 ? (int32_t)(units / kv_heads) : 1;
+  p.few.rows_log2 = p.tile.rows_log2 = -1;
   if (most_rows <= few_limit || head_size > 128) {
     // all requests in tiles of few rows (max_query_len may be wrong: any number of tiles each)
-    f.rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : few_limit;
-    f.max_rows = 0x7fffffff;
-    f.tiles = all_rows / f.rows + seqs;
+    const int rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : few_limit;
+    p.few.rows_log2 = log2_of(rows);
+    p.few.max_rows = 0x7fffffff;
+    p.waves = 4;
+    few_tiles = all_rows / rows + seqs;
   } else {
     // single tokens in one tile each, longer requests in large tiles
-    f.rows = group <= 16 ? 16 : group <= 32 ? 32 : few_limit;
-    f.max_rows = f.rows;
-    f.tiles = seqs;
-    t.min_rows = f.rows + 1;
-    t.max_rows = 0x7fffffff;
-    t.rows = all_rows / 256 * kv_heads >= units ? 256 : 128;
-    const int64_t chunks = seqs < all_rows / t.min_rows ? seqs : all_rows / t.min_rows;
-    t.tiles = all_rows / t.rows + chunks;
-    const int64_t fill = 2 * (int64_t)units / kv_heads;
-    plan_parts(t, t.tiles < fill ? (fill > 0 ? fill : 1) : 0, 512, seqs, capacity, kv_heads, head_size);
+    const int rows = group <= 16 ? 16 : few_limit;
+    p.few.rows_log2 = log2_of(rows);
+    p.few.max_rows = rows;
+    const int big = all_rows / 256 * kv_heads >= units / 2 ? 256 : 128;
+    p.waves = big / 32;
+    p.tile.rows_log2 = log2_of(big);
+    const int64_t chunks = seqs < all_rows / (rows + 1) ? seqs : all_rows / (rows + 1);
+    few_tiles = seqs;
+    chunk_tiles = all_rows / big + chunks;
+    // cut only where the tiles leave a quarter of the compute units idle: a part costs its state's
+    // way to memory and back
+    if (all_rows / big * kv_heads < units * 3 / 4) chunk_target = p.tile.fill;
+    p.tile.min_part = 512;
   }
-  if (f.tiles > all_rows) f.tiles = all_rows;
-  const int64_t fill = 2 * (int64_t)units / kv_heads;
-  plan_parts(f, fill > 0 ? fill : 1, 128, seqs, capacity, kv_heads, head_size);
+  if (few_tiles > all_rows) few_tiles = all_rows;
+  p.few.min_part = 128;
+  // workgroups of the mixed kernel take twice the waves, and its tiles even out what is left over
+  few_target = (p.tile.rows_log2 < 0 ? 4 : 1) * (int64_t)p.few.fill;
+  // cutting yields no more parts than the pages can fill
+  const int64_t most_few = few_tiles * (capacity / p.few.min_part);
+  if (few_target > most_few) few_target = most_few;
+  if (chunk_target > 0) {
+    const int64_t most = chunk_tiles * (capacity / p.tile.min_part);
+    if (chunk_target > most) chunk_target = most;
+  }
+  // every request is of one class: the tiles that are there at most
+  int64_t tiles = p.tile.rows_log2 < 0 ? few_tiles : (all_rows >> p.tile.rows_log2) + seqs;
+  if (tiles > all_rows) tiles = all_rows;
+  p.uncut_items = tiles;
+  p.items = tiles + few_target + chunk_target;
+  const int64_t chunk_rows = p.tile.rows_log2 < 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
+  const int64_t state_rows = chunk_rows + (((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
+  if (few_target + chunk_target == 0 || state_rows >= 0x7fffffffLL) return p;
+  p.few.target = (int32_t)few_target;
+  p.tile.target = (int32_t)chunk_target;
+  p.few.row_base = (int32_t)chunk_rows;
+  p.map_bytes = round256((2 * seqs + 1) * 4);
+  p.ml_bytes = round256(state_rows * 8);
+  p.o_bytes = round256(state_rows * head_size * 4);
   return p;
-}
-
-// Launches one class; `ws` is its part of the workspace or null.
-template <typename Launch>
-static int run_class(PagedAttnArgs a, const AttnClass& c, char* ws, int dtype, hipStream_t st,
-                     Launch launch) {
-  if (c.rows == 0) return SARATHI_OK;
-  a.min_rows = c.min_rows;
-  a.max_rows = c.max_rows;
-  const bool cut = c.target > 0 && ws;
-  if (cut) {
-    a.part_map = reinterpret_cast<int32_t*>(ws);
-    a.part_ml = reinterpret_cast<float*>(ws + c.map_bytes);
-    a.part_o = reinterpret_cast<float*>(ws + c.map_bytes + c.ml_bytes);
-    a.target = c.target;
-    a.min_part = c.min_part;
-  }
-  const int64_t groups = (cut ? c.items : c.tiles) * a.kv_heads;
-  if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
-  if (groups == 0) return SARATHI_OK;
-  const int rc = launch(a, groups);
-  if (rc != SARATHI_OK || !cut) return rc;
-  return dtype == kBF16 ? launch_join<kBF16>(a, c.rows, st) : launch_join<kF16>(a, c.rows, st);
 }
 
 }  // namespace sarathi_hip
 
 using namespace sarathi_hip;
+
+// Heads of up to 128 in batches that may hold chunks take the kernel that does both classes; the
+// others have few rows only.
+static int launch_paged_attn(const PagedAttnArgs& a, int dtype, int waves, bool page16, int64_t groups,
+                             hipStream_t st) {
+  if (groups == 0) return SARATHI_OK;
+  if (a.tile.rows_log2 < 0) return launch_attn_few(a, dtype, page16, groups, st);
+  if (dtype == kBF16)
+    return a.head_size <= 64 ? launch_attn_mixed_bf16_64(a, waves, page16, groups, st)
+                             : launch_attn_mixed_bf16_128(a, waves, page16, groups, st);
+  return a.head_size <= 64 ? launch_attn_mixed_f16_64(a, waves, page16, groups, st)
+                           : launch_attn_mixed_f16_128(a, waves, page16, groups, st);
+}
 
 static bool attn_sizes_ok(int64_t tokens, int64_t seqs, int64_t indices, int heads, int kv_heads,
                           int head_size, int page_size) {
@@ -556,7 +385,7 @@ extern "C" int64_t sarathi_paged_attention_workspace_bytes(int64_t num_tokens, i
     return 0;
   const AttnPlan p = plan_attention(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads,
                                     head_size, page_size, max_query_len);
-  return p.few.bytes() + p.tile.bytes();
+  return p.bytes();
 }
 
 extern "C" int sarathi_paged_attention(
@@ -628,16 +457,22 @@ extern "C" int sarathi_paged_attention(
     return launch_status();
   }
   // a workspace that is missing or too small means no cutting, not an error
-  char* ws = workspace && aligned16(workspace) && workspace_bytes >= p.few.bytes() + p.tile.bytes()
-                 ? reinterpret_cast<char*>(workspace)
-                 : nullptr;
-  int rc = run_class(a, p.tile, ws, dtype, st, [&](const PagedAttnArgs& x, int64_t groups) {
-    return launch_attn_tiles(x, dtype, p.tile.rows, groups, st);
-  });
-  if (rc != SARATHI_OK) return rc;
-  return run_class(a, p.few, ws ? ws + p.tile.bytes() : nullptr, dtype, st,
-                   [&](const PagedAttnArgs& x, int64_t groups) {
-                     return dtype == kBF16 ? launch_few_heads<kBF16>(x, p.few.rows / 16, groups, st)
-                                           : launch_few_heads<kF16>(x, p.few.rows / 16, groups, st);
-                   });
+  const bool cut = p.bytes() > 0 && workspace && aligned16(workspace) && workspace_bytes >= p.bytes();
+  a.few = p.few;
+  a.tile = p.tile;
+  if (cut) {
+    char* w = reinterpret_cast<char*>(workspace);
+    a.part_map = reinterpret_cast<int32_t*>(w);
+    a.part_ml = reinterpret_cast<float*>(w + p.map_bytes);
+    a.part_o = reinterpret_cast<float*>(w + p.map_bytes + p.ml_bytes);
+  } else {
+    a.few.target = a.tile.target = 0;
+  }
+  const int64_t groups = (cut ? p.items : p.uncut_items) * num_kv_heads;
+  if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
+  // offsets inside a share of sixteen keys are 32-bit
+  const bool page16 = page_size % 16 == 0 && a.entry_stride < (1 << 26);
+  const int rc = launch_paged_attn(a, dtype, p.waves, page16, groups, st);
+  if (rc != SARATHI_OK || !cut) return rc;
+  return dtype == kBF16 ? launch_join<kBF16>(a, st) : launch_join<kF16>(a, st);
 }

@@ -9,7 +9,7 @@
 // The query heads that share a key head are rows of the same product: a request's rows for one key
 // head are its new tokens times the G = heads / kv_heads query heads, token by token.
 //
-// Work items.  A kernel takes a request's rows in tiles and may cut the keys of a tile into parts
+// Work items.  The kernels take a request's rows in tiles and may cut the keys of a tile into parts
 // that different workgroups attend to; the parts' states are joined afterwards (the formula of
 // merge_attention_states).  Nothing is planned ahead: every workgroup sums up the requests' lengths
 // itself, arrives at the same part length and finds its own item, so a captured launch follows the
@@ -26,6 +26,16 @@ constexpr int kAttnMaxHead = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// How the requests of one class are cut into work items.
+struct AttnClass {
+  int32_t rows_log2;  // rows per tile; -1: the class is empty
+  int32_t max_rows;   // few: requests with more rows belong to the other class
+  int32_t target;     // items per key head that cutting stays below; 0: do not cut
+  int32_t fill;       // items per key head that fill the GPU once
+  int32_t min_part;   // least keys of a part, a multiple of 64
+  int32_t row_base;   // first state row of the class
+};
+
 struct PagedAttnArgs {
   const void* q;          // [T, heads, D], tokens q_stride elements apart
   const void* k_cache;
@@ -37,8 +47,8 @@ struct PagedAttnArgs {
   const int32_t* kv_indices;
   const int32_t* last_page_len;
   float* part_o;          // states of the parts, or null: nothing is cut
-  float* part_ml;         // [.. , 2]: running maximum (in powers of two) and sum
-  int32_t* part_map;      // [seqs + 1] first item, then [seqs] parts per tile
+  float* part_ml;         // [.. , 2]: reference (in powers of two) and sum
+  int32_t* part_map;      // [seqs] first state row, [seqs] parts per tile, and whether any is cut
   int64_t q_stride, out_stride;           // elements
   int64_t page_stride, entry_stride;      // bytes
   uint32_t page_magic;    // ceil(2^page_shift / page_size): division of positions by page_size
@@ -47,9 +57,7 @@ struct PagedAttnArgs {
   int32_t page_size, num_pages, num_indices;
   int32_t causal, window;                 // window < 0: none
   float scale_log2;                       // softmax scale * log2(e)
-  int32_t min_rows, max_rows;             // this kernel takes requests with rows in [min, max]
-  int32_t target;                         // items per key head that cutting aims at; 0: do not cut
-  int32_t min_part;                       // least keys of a part, a multiple of 64
+  AttnClass few, tile;                    // requests of up to few.max_rows rows; those of more
 };
 
 // One request as the kernels see it; whatever the index vectors hold, nothing outside the
@@ -97,12 +105,14 @@ SK_DEV int64_t attn_entry(const PagedAttnArgs& a, const AttnSeq& x, int32_t pos)
 
 // ---- work items ------------------------------------------------------------------------------
 
+constexpr int kPartKeys = 1024;
+
 struct AttnItem {
-  int32_t r;       // request, -1: none
-  int32_t tile;    // tile of its rows
-  int32_t part, parts;
-  int32_t index;   // item index over all requests: where the part's state goes
-  int32_t part_len;
+  int32_t r;         // request, -1: none
+  int32_t tiled;     // 1: a tile of a chunk, 0: a tile of few rows
+  int32_t tile;      // tile of its rows
+  int32_t part, parts, part_len;
+  int32_t state_row; // first state row of this tile and part (key head 0)
 };
 
 SK_DEV uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
@@ -114,92 +124,166 @@ SK_DEV uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
   return v;
 }
 
-// Most keys that a tile of the request spans with a window, counted from a multiple of 64.
-SK_DEV int32_t attn_window_keys(const PagedAttnArgs& a, const AttnSeq& x) {
+// Most keys that a tile of the request spans, counted from a multiple of 64 where a window cuts the
+// front off.
+SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
   const int64_t s = (int64_t)a.window + x.n + 63;
-  return s < x.s ? (int32_t)s : x.s;
+  return a.window >= 0 && s < x.s ? (int32_t)s : x.s;
 }
 
-// Rows per tile ROWS, WAVES waves in the workgroup.  `want` counts the items of one key head in
-// the order request, tile, part.  Two sums over the requests: keys times tiles, which fixes the
-// part length (the same for all, at least min_part, a multiple of 64, so that about a.target
-// items come out), and the number of items.  When nothing is cut the first is left out.  The
-// workgroup with `map` set leaves the item counts for the kernel that joins the parts.
-template <int ROWS, int WAVES>
+// Finds item `want` of a key head: first the tiles of the chunks, then those of few rows, each in
+// the order request, tile, part.  Two sums over the requests: keys times tiles of either class,
+// which fix the classes' part lengths, and the numbers of items.  A part is as long as filling the
+// GPU once allows but no longer than kPartKeys (below, its start and the way of its state to memory
+// and back weigh in), unless that made more than `target` items; it is at least min_part keys and a
+// multiple of 64.  When nothing is cut the first is left out.  The
+// workgroup with `map` set leaves the state rows for the kernel that joins the parts.  Sums of the
+// two classes share a word: tiles times keys stay far below 2^40 each in units of 64 keys, items
+// below 2^31.
+template <int WAVES>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
-  __shared__ uint64_t sums[WAVES];
+  __shared__ uint64_t sums[2][WAVES];
   __shared__ AttnItem found;
-  constexpr int NT = WAVES * 64;
+  constexpr int NT = WAVES * 64, KEEP = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t run = (a.seqs + NT - 1) / NT;
   const int64_t first = (int64_t)tid * run;
   const int32_t r0 = first < a.seqs ? (int32_t)first : a.seqs;
   const int32_t r1 = first + run < a.seqs ? (int32_t)(first + run) : a.seqs;
-  const bool narrow = a.seqs <= 64;  // all requests in the first wave's lanes: no exchange
-  int32_t part_len = 0x7fffffff;
-  auto tiles_of = [&](const AttnSeq& x) {
+  struct Load { int32_t tiles, keys; bool tiled; };
+  auto look = [&](int32_t r) {
+    const AttnSeq x = attn_seq(a, r);
     const int64_t rows = (int64_t)x.n * a.group;
-    return rows >= a.min_rows && rows <= a.max_rows ? (int32_t)((rows + ROWS - 1) / ROWS) : 0;
+    Load v;
+    v.tiled = a.few.rows_log2 < 0 || (a.tile.rows_log2 >= 0 && rows > a.few.max_rows);
+    const int32_t lg = v.tiled ? a.tile.rows_log2 : a.few.rows_log2;
+    v.tiles = (int32_t)((rows + ((int64_t)1 << lg) - 1) >> lg);
+    v.keys = attn_keys(a, x);
+    return v;
+  };
+  Load kept[KEEP];  // the first requests of this thread are looked at once
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) {
+    kept[i] = {0, 0, false};
+    if (r0 + i < r1) kept[i] = look(r0 + i);
+  }
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (r0 + i < r1) f(r0 + i, kept[i]);
+    for (int32_t r = r0 + KEEP; r < r1; ++r) f(r, look(r));
   };
   if (tid == 0) found.r = -1;
-  if (a.target > 0) {
-    uint64_t work = 0;
-    for (int32_t r = r0; r < r1; ++r) {
-      const AttnSeq x = attn_seq(a, r);
-      int32_t s = x.s;  // keys that the tiles of this request walk, roughly
-      if (a.window >= 0) s = attn_window_keys(a, x);
-      work += (uint64_t)tiles_of(x) * (uint32_t)s;
+  int32_t few_len = 0x7fffffff, tile_len = 0x7fffffff;
+  if (a.few.target > 0 || a.tile.target > 0) {
+    uint64_t few = 0, tile = 0;
+    each([&](int32_t, const Load& v) {
+      (v.tiled ? tile : few) += (uint64_t)v.tiles * (uint32_t)((v.keys + 63) >> 6);
+    });
+    few = wave_scan_u64(few, lane);
+    tile = wave_scan_u64(tile, lane);
+    if (lane == 63) {
+      sums[0][wave] = few;
+      sums[1][wave] = tile;
     }
-    work = wave_scan_u64(work, lane);
-    if (lane == 63) sums[wave] = work;
     __syncthreads();
-    work = 0;
+    few = tile = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) work += sums[w];
-    const uint64_t len = (work + (uint32_t)a.target - 1) / (uint32_t)a.target;
-    const uint64_t up = (len + 63) & ~63ull;
-    part_len = up > 0x3fffffc0ull ? 0x3fffffc0 : (int32_t)up;
-    if (part_len < a.min_part) part_len = a.min_part;
+    for (int w = 0; w < WAVES; ++w) {
+      few += sums[0][w];
+      tile += sums[1][w];
+    }
+    auto length = [](uint64_t work, const AttnClass& c) {
+      if (c.target <= 0) return 0x7fffffff;
+      uint64_t len = (work + (uint32_t)c.fill - 1) / (uint32_t)c.fill;
+      if (len > kPartKeys / 64) len = kPartKeys / 64;
+      const uint64_t least = (work + (uint32_t)c.target - 1) / (uint32_t)c.target;
+      if (len < least) len = least;
+      const int32_t keys = len > 0xffffffull ? 0x3fffffc0 : (int32_t)len * 64;
+      return keys > c.min_part ? keys : c.min_part;
+    };
+    few_len = length(few, a.few);
+    tile_len = length(tile, a.tile);
     __syncthreads();  // sums[] is written again below
   }
-  auto parts_of = [&](const AttnSeq& x) {
-    const int32_t s = a.window >= 0 ? attn_window_keys(a, x) : x.s;
-    return part_len == 0x7fffffff || s <= part_len ? 1 : (s - 1) / part_len + 1;
+  auto parts_of = [&](const Load& v) {
+    const int32_t len = v.tiled ? tile_len : few_len;
+    return v.keys <= len ? 1 : (v.keys - 1) / len + 1;
   };
+  // chunks' items in the upper half, those of few rows in the lower
   uint64_t mine = 0;
-  for (int32_t r = r0; r < r1; ++r) {
-    const AttnSeq x = attn_seq(a, r);
-    mine += (uint64_t)tiles_of(x) * (uint32_t)parts_of(x);
-  }
+  each([&](int32_t, const Load& v) {
+    mine += (uint64_t)(uint32_t)(v.tiles * parts_of(v)) << (v.tiled ? 32 : 0);
+  });
   const uint64_t incl = wave_scan_u64(mine, lane);
-  if (lane == 63) sums[wave] = incl;
+  if (lane == 63) sums[0][wave] = incl;
   __syncthreads();
-  uint64_t at = incl - mine;
-  if (!narrow)
-    for (int w = 0; w < wave; ++w) at += sums[w];
-  for (int32_t r = r0; r < r1; ++r) {
-    const AttnSeq x = attn_seq(a, r);
-    const int32_t parts = parts_of(x);
-    const uint64_t cnt = (uint64_t)tiles_of(x) * (uint32_t)parts;
+  uint64_t at = incl - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) at += sums[0][w];
+    all += sums[0][w];
+  }
+  // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
+  // are at work all the time; the last quarter of the few ones evens out the end.  Batch of 2304
+  // tokens: 876 us, 945 with all tiles first.
+  const uint32_t tile_items = (uint32_t)(all >> 32), few_items = (uint32_t)all;
+  const uint32_t mixed = tile_items + (uint32_t)((uint64_t)few_items * 3 / 4);
+  uint32_t tiles_before = tile_items;
+  bool tiled = false;
+  if (want < mixed) {
+    tiles_before = (uint32_t)(((uint64_t)want * tile_items + mixed - 1) / mixed);
+    tiled = (uint32_t)(((uint64_t)(want + 1) * tile_items + mixed - 1) / mixed) > tiles_before;
+  }
+  const uint32_t in_class = tiled ? tiles_before : want - tiles_before;
+  uint32_t tile_at = (uint32_t)(at >> 32), few_at = (uint32_t)at;
+  int32_t cut = 0;
+  each([&](int32_t r, const Load& v) {
+    const int32_t parts = parts_of(v);
+    const uint32_t cnt = (uint32_t)(v.tiles * parts);
+    uint32_t& mine_at = v.tiled ? tile_at : few_at;
+    const AttnClass& c = v.tiled ? a.tile : a.few;
+    const int32_t state = c.row_base + (int32_t)((mine_at * (uint32_t)a.kv_heads) << c.rows_log2);
     if (map) {
-      a.part_map[r] = (int32_t)at;
-      a.part_map[a.seqs + r] = cnt ? parts : 0;
+      a.part_map[r] = state;
+      a.part_map[a.seqs + r] = parts;
+      cut |= parts > 1;
     }
-    if (want >= at && want < at + cnt) {
-      const int32_t in = (int32_t)(want - at);
-      found = {r, in / parts, in % parts, parts, (int32_t)want, part_len};
+    if (v.tiled == tiled && in_class - mine_at < cnt) {
+      const int32_t in = (int32_t)(in_class - mine_at);
+      // a chunk's last tokens have the most keys: its last tile comes first
+      const int32_t tile = v.tiled ? v.tiles - 1 - in / parts : in / parts, part = in % parts;
+      found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
+               state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2)};
     }
-    at += cnt;
+    mine_at += cnt;
+  });
+  if (map) {  // uniform over the workgroup
+    cut = __syncthreads_or(cut);
+    if (tid == 0) a.part_map[2 * a.seqs] = cut;
   }
   __syncthreads();
-  AttnItem it = found;
-  it.r = __builtin_amdgcn_readfirstlane(it.r);
-  it.tile = __builtin_amdgcn_readfirstlane(it.tile);
-  it.part = __builtin_amdgcn_readfirstlane(it.part);
-  it.parts = __builtin_amdgcn_readfirstlane(it.parts);
-  it.index = __builtin_amdgcn_readfirstlane(it.index);
-  it.part_len = __builtin_amdgcn_readfirstlane(it.part_len);
+  AttnItem it;
+  it.r = __builtin_amdgcn_readfirstlane(found.r);
+  it.tiled = __builtin_amdgcn_readfirstlane(found.tiled);
+  it.tile = __builtin_amdgcn_readfirstlane(found.tile);
+  it.part = __builtin_amdgcn_readfirstlane(found.part);
+  it.parts = __builtin_amdgcn_readfirstlane(found.parts);
+  it.part_len = __builtin_amdgcn_readfirstlane(found.part_len);
+  it.state_row = __builtin_amdgcn_readfirstlane(found.state_row);
   return it;
+}
+
+// Keys [begin, end) of a part; keys are counted from a multiple of 64, so that sixteen of them lie
+// in one page where pages are multiples of 16.
+SK_DEV void attn_part(const AttnItem& it, int32_t span_lo, int32_t span_hi, int32_t& begin, int32_t& end) {
+  begin = span_lo & ~63;
+  end = span_hi;
+  if (it.parts > 1) {
+    const int64_t b = begin + (int64_t)it.part * it.part_len, e = b + it.part_len;
+    begin = b < span_hi ? (int32_t)b : span_hi;
+    end = e < span_hi ? (int32_t)e : span_hi;
+  }
 }
 
 // ---- matrix cores --------------------------------------------------------------------------------
@@ -232,52 +316,43 @@ template <int DT> SK_DEV f32x4 mfma16x16(u32x2 a, u32x2 b, f32x4 c) {
 }
 
 typedef __attribute__((address_space(3))) char lds_char;
-// Transposing reads: 16 lanes read four rows of sixteen 16-bit values, lane i the i % 4-th 8 bytes of
-// row i / 4, and receive column i: the values of the four rows.  N of them from byte addresses in
-// LDS, with their wait in the same block (the compiler's own form of this read waits for every load
-// into LDS that is in flight, also those of other buffers).
 SK_DEV uint32_t lds_addr(const lds_char* p) { return (uint32_t)(uintptr_t)p; }
-SK_DEV void lds_read_tr4(const uint32_t (&at)[4], u32x2 (&v)[4]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5\n\t"
-      "ds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
-      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
-      : "memory");
-}
-// One 16-byte (or 4-byte) piece per lane from global memory into LDS: lane l lands at base + 16 l
-// (4 l), base uniform over the wave; lanes that are off write nothing.  Completion counts in the
-// wave's vmcnt.
-template <int BYTES> SK_DEV void dma_to_lds(const void* src, lds_char* base) {
-  // (the builtin wants its size as a literal)
-  if constexpr (BYTES == 16)
-    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
-  else
-    __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 4, 0, 0);
-}
-
-// The same read for one address, its wait placed by the compiler; for kernels whose loads into LDS
-// are the ones below, of which the compiler knows nothing.
-SK_DEV u32x2 lds_read_tr_b64(const lds_char* p) {
+// Transposing read: 16 lanes read four rows of sixteen 16-bit values, lane i the i % 4-th 8 bytes of
+// row i / 4, and receive column i: the values of the four rows.
+SK_DEV u32x2 lds_read_tr_b64(uint32_t at) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (__attribute__((address_space(3))) s16x4*)p));
+                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)at));
 }
-// dma_to_lds() as instructions that the compiler does not look into: it places no waits for them, so
-// every read of what they bring stands behind a counted wait_vmcnt() (and a barrier, where another
-// wave loaded it).  No register is written but M0, which nothing else in those kernels uses.
-// `to` is the LDS address of the first lane, less `plus` (a constant).
-SK_DEV void dma_asm16(const void* src, uint32_t to, int plus) {
-  asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src), "n"(plus)
-               : "memory", "scc");
+SK_DEV u32x4 lds_read_b128(uint32_t at) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
 }
+// One 16-byte (or 4-byte) piece per lane from global memory into LDS: lane l lands at the base + 16 l
+// (4 l), the base uniform over the wave; lanes that are off write nothing.  Completion counts in the
+// wave's vmcnt.  Written as instructions that the compiler does not look into, because for its own
+// form of them it has the next transposing read wait for every load in flight.  So it places no waits
+// for them: every read of what they bring stands behind a counted wait_vmcnt() (and a barrier, where
+// another wave loaded it).  No register is written but M0, which nothing else in these kernels uses.
+// `to` is the LDS address of the first lane, less `plus` (a constant).  ONCE: data that no other
+// workgroup reads (non-temporal: 7.1 instead of 6.3 TB/s where a kernel does nothing but read).
+template <bool ONCE> SK_DEV void dma_asm16(const void* src, uint32_t to, int plus) {
+  if constexpr (ONCE)
+    asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(src),
+                 "n"(plus) : "memory", "scc");
+  else
+    asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(src),
+                 "n"(plus) : "memory", "scc");
+}
+template <bool ONCE>
 SK_DEV void dma_asm16(const char* uniform_base, uint32_t off, uint32_t to, int plus) {
-  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off),
-               "s"(uniform_base), "n"(plus)
-               : "memory", "scc");
+  if constexpr (ONCE)
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(off),
+                 "s"(uniform_base), "n"(plus) : "memory", "scc");
+  else
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off),
+                 "s"(uniform_base), "n"(plus) : "memory", "scc");
 }
-SK_DEV void dma_asm4(const void* src, lds_char* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_addr(base)), "v"(src)
-               : "memory");
+SK_DEV void dma_asm4(const void* src, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(src) : "memory");
 }
 // Meets the other waves; only LDS reads of this wave have to be complete (they are: their results
 // have been used).
@@ -297,7 +372,106 @@ SK_DEV float group_sum(float v) {
   return as_f32(b[0]) + as_f32(b[1]);
 }
 
-// lse of a state with maximum m (in powers of two) and sum l; -inf where nothing was seen
+// ---- loads of sixteen keys or values ---------------------------------------------------------------
+//
+// A share is sixteen consecutive keys (or values), the first at a multiple of 16, brought from
+// global memory straight into LDS by one wave: kDmas instructions of 1 KiB, whole rows of the head
+// side by side, 16-byte chunks swizzled within their row.  Keys outside [first, end) are never read:
+// the nearest one inside stands in (its score is masked).
+template <int DP> struct HeadShape {
+  static constexpr int kRowBytes = DP * 2;
+  static constexpr int kChunks = DP / 8;            // 16-byte chunks of a row
+  static constexpr int kRowsPerDma = 64 / kChunks;  // rows one load instruction moves
+  static constexpr int kDmas = 16 / kRowsPerDma;
+  static constexpr int kShareBytes = 16 * kRowBytes;
+};
+
+// PAD: the head is shorter than DP (chunks beyond it are not loaded).  PAGE16: pages of a multiple
+// of 16 keys, so that a share lies in one page and its address is scalar; the page number is a
+// scalar load that the caller issues ahead.  Otherwise page numbers, one per key, go through a small
+// LDS ring, loaded IDS / 2 shares ahead.  ONCE: no other workgroup reads these keys.
+template <int DP, bool PAD, bool PAGE16, int IDS, bool ONCE> struct ShareLoader {
+  using H = HeadShape<DP>;
+  const PagedAttnArgs& a;
+  const AttnSeq& x;
+  int32_t first, end;
+  int lane;
+  uint32_t ids;  // LDS address of this wave's page numbers, 64 bytes per share
+
+  SK_DEV int row_of(int n) const { return n * H::kRowsPerDma + lane / H::kChunks; }
+  // this lane's chunk of load n, with PAGE16 from the share's first entry on
+  template <typename Swz> SK_DEV uint32_t chunk(int n, Swz swz) const {
+    const uint32_t c = (uint32_t)((lane % H::kChunks) ^ swz(row_of(n))) * 16u;
+    return PAGE16 ? c + (uint32_t)row_of(n) * (uint32_t)a.entry_stride : c;
+  }
+  SK_DEV bool inside_head(int n, uint32_t c) const {
+    if constexpr (PAGE16) c -= (uint32_t)row_of(n) * (uint32_t)a.entry_stride;
+    return c < (uint32_t)a.head_size * 2u;
+  }
+  SK_DEV int32_t clamp_key(int32_t t) const { return t < first ? first : t < end ? t : end - 1; }
+  // the share at key t, or the nearest one that holds a key
+  SK_DEV int32_t base(int32_t t) const { return clamp_i32(t, first & ~15, (end - 1) & ~15); }
+  SK_DEV int32_t page(int32_t t) const {
+    return PAGE16 ? a.kv_indices[x.kv0 + attn_page_of(a, base(t))] : 0;
+  }
+  SK_DEV void load_ids(int32_t t, int32_t n) const {
+    if constexpr (!PAGE16) {
+      const int32_t* const from = a.kv_indices + x.kv0 + attn_page_of(a, clamp_key(t + (lane & 15)));
+      if (lane < 16) dma_asm4(from, ids + (uint32_t)n % IDS * 64u);
+    }
+  }
+  // share n at key t into LDS at to[r] for each of the R tensors src[r], chunks off[r][.]
+  template <int R>
+  SK_DEV void load(int32_t t, int32_t n, int32_t page, const char* const (&src)[R],
+                   const uint32_t (&off)[R][H::kDmas], const uint32_t (&to)[R]) const {
+    if constexpr (PAGE16) {
+      const int32_t t0 = base(t);
+      const int64_t e = attn_clip_page(a, page) * a.page_stride +
+                        (int64_t)(t0 - attn_page_of(a, t0) * a.page_size) * a.entry_stride;
+      const bool whole = t0 >= first && t0 + 16 <= end;  // uniform over the wave
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const char* const from = src[r] + e;
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < H::kDmas; ++i)
+            if (!PAD || inside_head(i, off[r][i])) dma_asm16<ONCE>(from, off[r][i], to[r], i * 1024);
+        } else {
+#pragma unroll
+          for (int i = 0; i < H::kDmas; ++i) {
+            const int32_t row = clamp_key(t0 + row_of(i)) - t0;
+            if (!PAD || inside_head(i, off[r][i]))
+              dma_asm16<ONCE>(from, off[r][i] + (uint32_t)(row - row_of(i)) * (uint32_t)a.entry_stride, to[r],
+                        i * 1024);
+          }
+        }
+      }
+    } else {
+      const int32_t key = clamp_key(t + (lane & 15));
+      page = *(const __attribute__((address_space(3))) int32_t*)(uintptr_t)(
+          ids + (uint32_t)n % IDS * 64u + (uint32_t)(lane & 15) * 4u);
+      const int64_t e = attn_clip_page(a, page) * a.page_stride +
+                        (int64_t)(key - attn_page_of(a, key) * a.page_size) * a.entry_stride;
+      const int32_t e_lo = (int32_t)e, e_hi = (int32_t)(e >> 32);
+#pragma unroll
+      for (int i = 0; i < H::kDmas; ++i) {
+        const int64_t s = (int64_t)(((uint64_t)(uint32_t)__shfl(e_hi, row_of(i), 64) << 32) |
+                                    (uint32_t)__shfl(e_lo, row_of(i), 64));
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (!PAD || inside_head(i, off[r][i])) dma_asm16<ONCE>(src[r] + s + off[r][i], to[r], i * 1024);
+      }
+    }
+  }
+};
+
+// The running maximum of a row is only a reference for its exponents, and it is raised only when a
+// score passes it by more than 2^kRaise: probabilities then stay below 2^8, which neither 16-bit type
+// nor the 32-bit sums mind, and the output is almost never rescaled.
+constexpr float kRefStart = -3.0e38f;  // below every score; finite, so that no difference is undefined
+constexpr float kRaise = 8.f;
+
+// lse of a state with reference m (in powers of two) and sum l; -inf where nothing was seen
 SK_DEV float attn_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
 
 }  // namespace sarathi_hip
