@@ -323,13 +323,16 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   p.few.min_part = 128;
   // workgroups of the mixed kernel take twice the waves, and its tiles even out what is left over
   few_target = (p.tile.rows_log2 < 0 ? 4 : 1) * (int64_t)p.few.fill;
-  // cutting yields no more parts than the pages can fill
-  const int64_t most_few = few_tiles * (capacity / p.few.min_part);
-  if (few_target > most_few) few_target = most_few;
-  if (chunk_target > 0) {
-    const int64_t most = chunk_tiles * (capacity / p.tile.min_part);
-    if (chunk_target > most) chunk_target = most;
-  }
+  // Cutting yields no more parts than the pages can fill, and where parts are as long as filling the
+  // GPU once allows, no more than that takes: the fewer workgroups find nothing to do, the better.
+  auto bound = [&](int64_t target, const AttnClass& c, int64_t tiles) {
+    const int64_t keys = ((most_rows >> c.rows_log2) + 1) * capacity;  // at most so many, times tiles
+    int64_t most = keys / kPartKeys > c.fill ? keys / kPartKeys : c.fill;
+    if (most > tiles * (capacity / c.min_part)) most = tiles * (capacity / c.min_part);
+    return target < most ? target : most;
+  };
+  few_target = bound(few_target, p.few, few_tiles);
+  if (chunk_target > 0) chunk_target = bound(chunk_target, p.tile, chunk_tiles);
   // every request is of one class: the tiles that are there at most
   int64_t tiles = p.tile.rows_log2 < 0 ? few_tiles : (all_rows >> p.tile.rows_log2) + seqs;
   if (tiles > all_rows) tiles = all_rows;

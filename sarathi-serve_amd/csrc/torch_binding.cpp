@@ -9,15 +9,18 @@
 // torch's current HIP stream for it; (c) forwards raw pointers, sizes and
 // strides to the C ABI of include/sarathi_ops.h and turns a non-zero status
 // into a RuntimeError.  It never copies or synchronises, and allocates only the scratch
-// tensor that moe_align_block_size uses for inputs above 32 K ids and, once per (device, stream),
-// the four-byte completion counter of fused_topk_align.
+// tensors that moe_align_block_size uses for inputs above 32 K ids and paged_attention for cut
+// contexts, the outputs of the ops that return theirs and, once per (device, stream), the four-byte
+// completion counter of fused_topk_align.
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "../../include/sarathi_ops.h"
 
@@ -398,64 +401,76 @@ void rotary_embedding_append_paged_kv(torch::Tensor& positions, torch::Tensor& q
            op);
 }
 
+// A contiguous view of `n` elements of `flat` from `at` on, made without the dispatcher (the ops that
+// return several small vectors are bound by what the host does).
+torch::Tensor part_of(const torch::Tensor& flat, int64_t at, int64_t n) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  t.unsafeGetTensorImpl()->set_storage_offset(at);
+  return t;
+}
+
 // the index vectors of a batch from its lengths; see include/sarathi_ops.h for what they hold
-void build_paged_kv_metadata(torch::Tensor& query_lens, torch::Tensor& seq_lens,
-                             torch::Tensor& block_tables, torch::Tensor& qo_indptr,
-                             torch::Tensor& kv_indptr, torch::Tensor& kv_indices,
-                             torch::Tensor& kv_last_page_len, torch::Tensor& batch_indices,
-                             torch::Tensor& positions, torch::Tensor& slot_mapping,
-                             torch::Tensor& rope_positions, int64_t page_size) {
+std::vector<torch::Tensor> build_paged_kv_metadata(
+    const torch::Tensor& query_lens, const torch::Tensor& seq_lens, const torch::Tensor& block_tables,
+    int64_t page_size, int64_t num_tokens, int64_t num_kv_pages) {
   const char* op = "build_paged_kv_metadata";
   check_i32(query_lens, query_lens, op, "query_lens");
   check_i32(seq_lens, query_lens, op, "seq_lens");
   check_gpu(block_tables, query_lens, op, "block_tables");
-  check_i32(qo_indptr, query_lens, op, "qo_indptr");
-  check_i32(kv_indptr, query_lens, op, "kv_indptr");
-  check_i32(kv_indices, query_lens, op, "kv_indices");
-  check_i32(kv_last_page_len, query_lens, op, "kv_last_page_len");
-  check_i32(batch_indices, query_lens, op, "batch_indices");
-  check_i32(positions, query_lens, op, "positions");
-  check_i32(slot_mapping, query_lens, op, "slot_mapping");
-  check_gpu(rope_positions, query_lens, op, "rope_positions");
-  const int64_t n = query_lens.numel(), t = positions.numel();
+  const int64_t n = query_lens.numel();
   TORCH_CHECK(page_size > 0 && page_size <= INT32_MAX, op, ": page_size must be positive");
-  TORCH_CHECK(seq_lens.numel() == n && kv_last_page_len.numel() == n && qo_indptr.numel() == n + 1 &&
-                  kv_indptr.numel() == n + 1,
-              op, ": expected query_lens, seq_lens and kv_last_page_len [n], qo_indptr and kv_indptr [n+1]");
+  TORCH_CHECK(num_tokens >= 0 && num_tokens < INT32_MAX && num_kv_pages >= 0 && num_kv_pages < INT32_MAX,
+              op, ": num_tokens and num_kv_pages must not be negative and fit 32 bits");
+  TORCH_CHECK(seq_lens.numel() == n, op, ": query_lens and seq_lens must be of one length");
   TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == n &&
                   block_tables.scalar_type() == at::ScalarType::Int &&
                   (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
               op, ": block_tables must be int32 [num_seqs, max_pages] with contiguous rows");
   TORCH_CHECK(n <= 1 || block_tables.stride(0) >= block_tables.size(1), op,
               ": the rows of block_tables must not overlap");
-  TORCH_CHECK(batch_indices.numel() == t && slot_mapping.numel() == t && rope_positions.numel() == t &&
-                  rope_positions.scalar_type() == at::ScalarType::Long && rope_positions.is_contiguous(),
-              op, ": the per-token vectors must hold num_tokens entries, rope_positions int64");
   LaunchScope scope(query_lens);
+  // one allocation; the 64-bit vector first, for its alignment
+  const torch::Tensor flat =
+      torch::empty({5 * num_tokens + num_kv_pages + 3 * n + 2}, query_lens.options());
+  int64_t at = 2 * num_tokens;
+  auto take = [&](int64_t len) {
+    torch::Tensor t = part_of(flat, at, len);
+    at += len;
+    return t;
+  };
+  std::vector<torch::Tensor> out;
+  out.reserve(8);
+  for (int64_t len : {n + 1, n + 1, num_kv_pages, n, num_tokens, num_tokens, num_tokens})
+    out.push_back(take(len));
+  auto rope = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(),
+                                                       caffe2::TypeMeta::Make<int64_t>());
+  rope.unsafeGetTensorImpl()->set_sizes_contiguous({num_tokens});
+  out.push_back(rope);
+  auto i32 = [&](int i) { return out[i].data_ptr<int32_t>(); };
   raise_on(sarathi_build_paged_kv_metadata(
                query_lens.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
-               block_tables.data_ptr<int32_t>(), qo_indptr.data_ptr<int32_t>(),
-               kv_indptr.data_ptr<int32_t>(), kv_indices.data_ptr<int32_t>(),
-               kv_last_page_len.data_ptr<int32_t>(), batch_indices.data_ptr<int32_t>(),
-               positions.data_ptr<int32_t>(), slot_mapping.data_ptr<int32_t>(),
-               rope_positions.data_ptr<int64_t>(), n, block_tables.size(1),
-               n > 1 ? block_tables.stride(0) : block_tables.size(1), (int)page_size, t,
-               kv_indices.numel(), scope.stream),
+               block_tables.data_ptr<int32_t>(), i32(0), i32(1), i32(2), i32(3), i32(4), i32(5), i32(6),
+               out[7].data_ptr<int64_t>(), n, block_tables.size(1),
+               n > 1 ? block_tables.stride(0) : block_tables.size(1), (int)page_size, num_tokens,
+               num_kv_pages, scope.stream),
            op);
+  return out;
 }
 
-// attention of the batch's new tokens over the paged cache.  The scratch for cut contexts comes from
-// torch's caching allocator on the launch stream, so calls never share it.
-void paged_attention(torch::Tensor& query, torch::Tensor& k_cache, torch::Tensor& v_cache,
-                     torch::Tensor& qo_indptr, torch::Tensor& kv_indptr, torch::Tensor& kv_indices,
-                     torch::Tensor& kv_last_page_len, torch::Tensor& out,
-                     c10::optional<torch::Tensor> lse, double sm_scale, bool causal,
-                     int64_t window_left, int64_t max_query_len) {
+// Attention of the batch's new tokens over the paged cache, a (K, V) pair or (v_cache empty) the
+// joint [num_pages, 2, page_size, heads, head_size] tensor.  Returns out, and lse where asked for.
+// The scratch for cut contexts comes from torch's caching allocator on the launch stream, so calls
+// never share it.
+std::vector<torch::Tensor> paged_attention(
+    const torch::Tensor& query, const torch::Tensor& cache, const c10::optional<torch::Tensor>& v_cache,
+    const torch::Tensor& qo_indptr, const torch::Tensor& kv_indptr, const torch::Tensor& kv_indices,
+    const torch::Tensor& kv_last_page_len, const c10::optional<torch::Tensor>& out_or_none,
+    bool return_lse, const c10::optional<double>& sm_scale, bool causal, int64_t window_left,
+    int64_t max_query_len) {
   const char* op = "paged_attention";
   check_gpu(query, query, op, "query");
-  check_gpu(k_cache, query, op, "k_cache");
-  check_gpu(v_cache, query, op, "v_cache");
-  check_gpu(out, query, op, "out");
+  check_gpu(cache, query, op, v_cache.has_value() ? "k_cache" : "paged_kv_cache");
   check_i32(qo_indptr, query, op, "qo_indptr");
   check_i32(kv_indptr, query, op, "kv_indptr");
   check_i32(kv_indices, query, op, "kv_indices");
@@ -463,62 +478,79 @@ void paged_attention(torch::Tensor& query, torch::Tensor& k_cache, torch::Tensor
   TORCH_CHECK(query.scalar_type() == at::ScalarType::Half ||
                   query.scalar_type() == at::ScalarType::BFloat16,
               op, ": only bfloat16 and float16 are supported, got ", query.scalar_type());
-  TORCH_CHECK(k_cache.scalar_type() == query.scalar_type() &&
-                  v_cache.scalar_type() == query.scalar_type() &&
-                  out.scalar_type() == query.scalar_type(),
-              op, ": query, out and the cache must share a dtype");
-  const PagedGeom g = paged_geom(k_cache, v_cache, op);
-  TORCH_CHECK(g.heads > 0 && g.head_size > 0 && g.page_size > 0, op, ": the cache has no entries");
+  TORCH_CHECK(cache.scalar_type() == query.scalar_type(), op, ": query and the cache must share a dtype");
+  PagedGeom g;
+  const char* k_ptr = static_cast<const char*>(cache.data_ptr());
+  const char* v_ptr;
+  if (v_cache.has_value()) {
+    check_gpu(*v_cache, query, op, "v_cache");
+    g = paged_geom(cache, *v_cache, op);
+    v_ptr = static_cast<const char*>(v_cache->data_ptr());
+  } else {
+    TORCH_CHECK(cache.dim() == 5 && cache.size(1) == 2, op,
+                ": paged_kv_cache must be [num_pages, 2, page_size, num_kv_heads, head_size]");
+    TORCH_CHECK(cache.stride(4) == 1 && cache.stride(3) == cache.size(4), op,
+                ": the [num_kv_heads, head_size] part of a cache entry must be contiguous");
+    g = {cache.size(2), cache.size(3), cache.size(4), cache.stride(0), cache.stride(2)};
+    v_ptr = k_ptr + cache.stride(1) * cache.element_size();
+  }
+  TORCH_CHECK(g.heads > 0 && g.head_size > 0 && g.page_size > 0 && g.page_size <= INT32_MAX, op,
+              ": the cache must have entries");
   TORCH_CHECK(g.head_size <= 256, op, ": head_size must be at most 256, got ", g.head_size);
   TORCH_CHECK(query.dim() == 2 || query.dim() == 3, op,
               ": query must be [tokens, heads, head_size] or [tokens, heads * head_size]");
   const int64_t width = query.dim() == 2 ? query.size(1) : query.size(1) * query.size(2);
   TORCH_CHECK(width > 0 && width % (g.heads * g.head_size) == 0, op,
-              ": the query heads must be a multiple of the cache's ", g.heads, " heads of ",
-              g.head_size);
+              ": the query heads must be a multiple of the cache's ", g.heads, " heads of ", g.head_size);
   const int64_t qs = token_rows(query, width, g.head_size, op, "query");
-  TORCH_CHECK(out.sizes() == query.sizes(), op, ": out and query shapes differ");
-  const int64_t os = token_rows(out, width, g.head_size, op, "out");
   const int64_t tokens = query.size(0), heads = width / g.head_size;
   const int64_t seqs = kv_last_page_len.numel();
+  TORCH_CHECK(heads <= 65535, op, ": at most 65535 query heads");
   TORCH_CHECK(qo_indptr.numel() == seqs + 1 && kv_indptr.numel() == seqs + 1, op,
               ": expected qo_indptr and kv_indptr [n+1], kv_last_page_len [n]");
-  TORCH_CHECK(tokens <= 1 || (qs >= width && os >= width), op, ": rows must not overlap");
-  float* lse_ptr = nullptr;
-  if (lse.has_value()) {
-    check_gpu(*lse, query, op, "lse");
-    TORCH_CHECK(lse->scalar_type() == at::ScalarType::Float && lse->is_contiguous() &&
-                    lse->dim() == 2 && lse->size(0) == tokens && lse->size(1) == heads,
-                op, ": lse must be contiguous float32 [tokens, heads]");
-    lse_ptr = lse->data_ptr<float>();
-  }
   TORCH_CHECK(max_query_len >= 0, op, ": max_query_len must not be negative");
-  TORCH_CHECK(heads <= 65535 && g.page_size <= INT32_MAX, op, ": too many heads or entries");
   LaunchScope scope(query);
+  torch::Tensor out;
+  if (out_or_none.has_value()) {
+    out = *out_or_none;
+    check_gpu(out, query, op, "out");
+    TORCH_CHECK(out.scalar_type() == query.scalar_type() && out.sizes() == query.sizes(), op,
+                ": out must have query's dtype and shape");
+  } else {
+    out = torch::empty(query.sizes(), query.options());
+  }
+  const int64_t os = token_rows(out, width, g.head_size, op, "out");
+  TORCH_CHECK(tokens <= 1 || (qs >= width && os >= width), op, ": rows must not overlap");
+  std::vector<torch::Tensor> result = {out};
+  float* lse = nullptr;
+  if (return_lse) {
+    result.push_back(torch::empty({tokens, heads}, query.options().dtype(torch::kFloat)));
+    lse = result[1].data_ptr<float>();
+  }
   const int64_t ws = sarathi_paged_attention_workspace_bytes(
       tokens, seqs, kv_indices.numel(), (int)heads, (int)g.heads, (int)g.head_size,
       (int)g.page_size, max_query_len);
   torch::Tensor workspace;
   if (ws > 0) workspace = torch::empty({ws}, query.options().dtype(torch::kUInt8));
+  const double scale = sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt((double)g.head_size);
   raise_on(sarathi_paged_attention(
-               query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse_ptr,
-               qo_indptr.data_ptr<int32_t>(), kv_indptr.data_ptr<int32_t>(),
-               kv_indices.data_ptr<int32_t>(), kv_last_page_len.data_ptr<int32_t>(), tokens, seqs,
-               kv_indices.numel(), k_cache.size(0), (int)heads, (int)g.heads, (int)g.head_size,
-               (int)g.page_size, tokens > 1 ? qs : width, tokens > 1 ? os : width, g.page_stride,
-               g.entry_stride, (float)sm_scale, causal ? 1 : 0, window_left, max_query_len,
-               ws > 0 ? workspace.data_ptr() : nullptr, ws, dtype_code(query, op), scope.stream),
+               query.data_ptr(), k_ptr, v_ptr, out.data_ptr(), lse, qo_indptr.data_ptr<int32_t>(),
+               kv_indptr.data_ptr<int32_t>(), kv_indices.data_ptr<int32_t>(),
+               kv_last_page_len.data_ptr<int32_t>(), tokens, seqs, kv_indices.numel(), cache.size(0),
+               (int)heads, (int)g.heads, (int)g.head_size, (int)g.page_size, tokens > 1 ? qs : width,
+               tokens > 1 ? os : width, g.page_stride, g.entry_stride, (float)scale, causal ? 1 : 0,
+               window_left, max_query_len, ws > 0 ? workspace.data_ptr() : nullptr, ws,
+               dtype_code(query, op), scope.stream),
            op);
+  return result;
 }
 
 // joins states [S, T, H, D] with their lse [S, T, H]; the state and token dimensions may have any
 // strides
-void merge_attention_states(torch::Tensor& v, torch::Tensor& lse, torch::Tensor& out,
-                            c10::optional<torch::Tensor> out_lse) {
+std::vector<torch::Tensor> merge_attention_states(const torch::Tensor& v, const torch::Tensor& lse) {
   const char* op = "merge_attention_states";
   check_gpu(v, v, op, "v");
   check_gpu(lse, v, op, "lse");
-  check_gpu(out, v, op, "out");
   const int code = dtype_code(v, op);
   TORCH_CHECK(v.dim() == 4 && lse.dim() == 3 && lse.size(0) == v.size(0) && lse.size(1) == v.size(1) &&
                   lse.size(2) == v.size(2),
@@ -529,25 +561,17 @@ void merge_attention_states(torch::Tensor& v, torch::Tensor& lse, torch::Tensor&
               ": the [heads, head_size] part of v must be contiguous");
   TORCH_CHECK(lse.scalar_type() == at::ScalarType::Float && (lse.stride(2) == 1 || H == 1), op,
               ": lse must be float32 with contiguous heads");
-  TORCH_CHECK(out.dim() == 3 && out.size(0) == T && out.size(1) == H && out.size(2) == D &&
-                  out.is_contiguous() && out.scalar_type() == v.scalar_type(),
-              op, ": out must be contiguous [tokens, heads, head_size] of v's dtype");
   TORCH_CHECK(T <= 1 || (v.stride(1) >= H * D && lse.stride(1) >= H), op, ": rows must not overlap");
-  float* out_lse_ptr = nullptr;
-  if (out_lse.has_value()) {
-    check_gpu(*out_lse, v, op, "out_lse");
-    TORCH_CHECK(out_lse->scalar_type() == at::ScalarType::Float && out_lse->is_contiguous() &&
-                    out_lse->dim() == 2 && out_lse->size(0) == T && out_lse->size(1) == H,
-                op, ": out_lse must be contiguous float32 [tokens, heads]");
-    out_lse_ptr = out_lse->data_ptr<float>();
-  }
   TORCH_CHECK(H <= INT32_MAX && D <= INT32_MAX, op, ": too many heads or elements");
   LaunchScope scope(v);
+  const torch::Tensor out = torch::empty({T, H, D}, v.options());
+  const torch::Tensor out_lse = torch::empty({T, H}, lse.options());
   raise_on(sarathi_merge_attention_states(
-               v.data_ptr(), lse.data_ptr<float>(), out.data_ptr(), out_lse_ptr, S, T, (int)H, (int)D,
-               v.stride(0), T > 1 ? v.stride(1) : H * D, lse.stride(0), T > 1 ? lse.stride(1) : H,
-               H * D, H, code, scope.stream),
+               v.data_ptr(), lse.data_ptr<float>(), out.data_ptr(), out_lse.data_ptr<float>(), S, T,
+               (int)H, (int)D, v.stride(0), T > 1 ? v.stride(1) : H * D, lse.stride(0),
+               T > 1 ? lse.stride(1) : H, H * D, H, code, scope.stream),
            op);
+  return {out, out_lse};
 }
 
 // ---- moe_ops -----------------------------------------------------------------
@@ -984,22 +1008,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         pybind11::arg("kv_indptr"), pybind11::arg("num_append_tokens"),
         pybind11::arg("write_key"), pybind11::arg("slot_mapping") = pybind11::none());
   m.def("build_paged_kv_metadata", &build_paged_kv_metadata,
-        "index vectors of a hybrid batch from its lengths and page tables",
-        pybind11::arg("query_lens"), pybind11::arg("seq_lens"), pybind11::arg("block_tables"),
-        pybind11::arg("qo_indptr"), pybind11::arg("kv_indptr"), pybind11::arg("kv_indices"),
-        pybind11::arg("kv_last_page_len"), pybind11::arg("batch_indices"),
-        pybind11::arg("positions"), pybind11::arg("slot_mapping"), pybind11::arg("rope_positions"),
-        pybind11::arg("page_size"));
+        "index vectors of a hybrid batch from its lengths and page tables");
   m.def("paged_attention", &paged_attention,
-        "attention of a hybrid batch's new tokens over a paged (NHD) KV cache",
-        pybind11::arg("query"), pybind11::arg("k_cache"), pybind11::arg("v_cache"),
-        pybind11::arg("qo_indptr"), pybind11::arg("kv_indptr"), pybind11::arg("kv_indices"),
-        pybind11::arg("kv_last_page_len"), pybind11::arg("out"), pybind11::arg("lse"),
-        pybind11::arg("sm_scale"), pybind11::arg("causal") = true,
-        pybind11::arg("window_left") = -1, pybind11::arg("max_query_len") = 0);
+        "attention of a hybrid batch's new tokens over a paged (NHD) KV cache");
   m.def("merge_attention_states", &merge_attention_states,
-        "join attention states computed over disjoint parts of a context", pybind11::arg("v"),
-        pybind11::arg("lse"), pybind11::arg("out"), pybind11::arg("out_lse") = pybind11::none());
+        "join attention states computed over disjoint parts of a context");
   // moe_ops
   m.def("topk_softmax", &topk_softmax, "softmax over experts + top-k (raw probabilities)");
   m.def("topk_softmax_renorm", &topk_softmax_renorm,

@@ -118,18 +118,8 @@ def build_paged_kv_metadata(query_lens: torch.Tensor, seq_lens: torch.Tensor,
     (``rope_positions``: 0), and the append ops skip negative slots and positions."""
     if num_kv_pages is None:
         num_kv_pages = block_tables.numel()
-    if num_tokens < 0 or num_kv_pages < 0:
-        raise ValueError("num_tokens and num_kv_pages must not be negative")
-    if page_size <= 0:
-        raise ValueError("page_size must be positive")
-    seqs = query_lens.numel()
-    # one allocation for the seven int32 vectors
-    sizes = [seqs + 1, seqs + 1, num_kv_pages, seqs, num_tokens, num_tokens, num_tokens]
-    flat = torch.empty((sum(sizes),), dtype=torch.int32, device=query_lens.device)
-    meta = PagedKvMetadata(*flat.split(sizes),
-                           torch.empty((num_tokens,), dtype=torch.int64, device=query_lens.device))
-    _C.build_paged_kv_metadata(query_lens, seq_lens, block_tables, *meta, page_size)
-    return meta
+    return PagedKvMetadata._make(_C.build_paged_kv_metadata(query_lens, seq_lens, block_tables, page_size,
+                                                            num_tokens, num_kv_pages))
 
 
 def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: torch.Tensor,
@@ -152,18 +142,16 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: 
     Returns ``out`` (shaped like ``query``), with ``return_lse`` also the natural-log sums
     ``[num_tokens, num_heads]`` (float32) that ``merge_attention_states`` joins.  A token that sees no
     key gets 0 and -inf; rows behind the last request are not written."""
-    k_cache, v_cache = _split_cache(paged_kv_cache, kv_layout)
-    if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    head_size = k_cache.shape[-1]
-    lse = None
-    if return_lse:
-        heads = query.shape[1] // head_size if query.dim() == 2 else query.shape[1]
-        lse = torch.empty((query.shape[0], heads), dtype=torch.float32, device=query.device)
-    _C.paged_attention(query, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
-                       out, lse, head_size ** -0.5 if sm_scale is None else sm_scale, causal,
-                       window_left, 0 if max_query_len is None else max_query_len)
-    return (out, lse) if return_lse else out
+    if kv_layout != "NHD":
+        raise ValueError("only the NHD page layout is supported, got %r" % (kv_layout,))
+    if isinstance(paged_kv_cache, (tuple, list)):
+        k_cache, v_cache = paged_kv_cache
+    else:
+        k_cache, v_cache = paged_kv_cache, None
+    result = _C.paged_attention(query, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, kv_last_page_len,
+                                out, return_lse, sm_scale, causal, window_left,
+                                0 if max_query_len is None else max_query_len)
+    return tuple(result) if return_lse else result[0]
 
 
 def merge_attention_states(v: torch.Tensor, lse: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -171,9 +159,7 @@ def merge_attention_states(v: torch.Tensor, lse: torch.Tensor) -> Tuple[torch.Te
     share and each request's own suffix: ``v`` ``[states, tokens, heads, head_size]``, ``lse``
     ``[states, tokens, heads]`` (natural log, float32).  The state and token dimensions may have any
     strides.  Returns the joined output and its lse; states with lse -inf are left out."""
-    out = torch.empty(v.shape[1:], dtype=v.dtype, device=v.device)
-    out_lse = torch.empty(lse.shape[1:], dtype=torch.float32, device=v.device)
-    _C.merge_attention_states(v, lse, out, out_lse)
+    out, out_lse = _C.merge_attention_states(v, lse)
     return out, out_lse
 
 
