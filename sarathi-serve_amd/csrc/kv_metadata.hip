@@ -11,19 +11,20 @@
 //   page * page_size + entry of that position, and the position again as the rotary embedding's
 //   64-bit index.
 //
-// The work is a prefix sum over the requests and then one lookup per token and per page: a few
-// hundred KiB at the most, so what bounds it is latency.  Up to kMetaLdsSeqs requests it is ONE
-// launch of independent workgroups: each of them adds up all the lengths itself (they come out of
-// L2; 1008 requests cost about a microsecond), keeps both prefix arrays in LDS and looks its own
-// tokens and pages up there.  More requests take two launches, a scan by one workgroup and then
-// the lookups against the prefix arrays in global memory.
+// The work is a sum over the requests in front of one's own and then one lookup per token and per
+// page; what bounds it is latency, then the bytes of the page table.  Up to kMetaOneLaunch requests it
+// is ONE launch of independent workgroups, each of one request (or of a piece of a long one): it adds
+// up the lengths of the requests before its own (all of them come out of L2), and then its tokens and
+// pages lie side by side, so nothing is searched for.  The additions grow with the square of the
+// requests; beyond the limit one workgroup writes the prefix sums first.
 #include "launch.h"
 #include "vec16.h"
 
 namespace sarathi_hip {
 
-constexpr int kMetaLdsSeqs = 4096;   // two prefix arrays of 16 KiB
-constexpr int kMetaPerThread = 4;    // tokens or pages a thread looks up
+constexpr int kMetaOneLaunch = 4096;
+constexpr int kMetaPiece = 2048;  // tokens or pages of a request that one workgroup takes
+constexpr int kMetaFill = 16;     // workgroups that fill the room behind the batch
 
 struct KvMetaArgs {
   const int32_t* query_lens;
@@ -35,7 +36,7 @@ struct KvMetaArgs {
   int64_t table_stride;   // entries between the rows of the table
   int32_t seqs, max_pages, page_size;
   int64_t num_tokens, num_pages;   // room in the per-token vectors, resp. in kv_indices
-  uint32_t token_groups;           // workgroups that work on tokens; the others work on pages
+  uint32_t pieces;                 // workgroups per request
 };
 
 SK_DEV int32_t meta_new(const KvMetaArgs& a, int32_t r) {
@@ -108,78 +109,93 @@ SK_DEV void meta_write_request(const KvMetaArgs& a, int32_t r, int64_t q, int64_
   a.last_page_len[r] = last;
 }
 
-// The request whose range of `starts` holds i: starts[lo] <= i < starts[hi].  Empty requests
-// (repeated entries) are stepped over.  i lies below starts[seqs].
-SK_DEV int32_t meta_find(const int32_t* starts, int32_t seqs, int64_t i) {
-  int32_t lo = 0, hi = seqs;
-  while (hi - lo > 1) {
-    const int32_t mid = (int32_t)(((uint32_t)lo + (uint32_t)hi) >> 1);
-    if (starts[mid] <= i) lo = mid; else hi = mid;
+// Sums over the workgroup's 256 threads; every thread returns them.
+SK_DEV void meta_block_sum(int64_t& q, int64_t& p) {
+  __shared__ int64_t sums[4][2];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    q += __shfl_xor(q, d, 64);
+    p += __shfl_xor(p, d, 64);
   }
-  return lo;
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x >> 6][0] = q;
+    sums[threadIdx.x >> 6][1] = p;
+  }
+  __syncthreads();
+  q = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
+  p = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
 }
 
-SK_DEV void meta_lookups(const KvMetaArgs& a, const int32_t* qo, const int32_t* kv) {
-  const bool is_token = blockIdx.x < a.token_groups;  // uniform over the workgroup
-  const int64_t group = is_token ? blockIdx.x : blockIdx.x - a.token_groups;
-  const int64_t base = group * (256 * kMetaPerThread) + threadIdx.x;
-  if (is_token) {
-    const int32_t total = qo[a.seqs];
-#pragma unroll
-    for (int k = 0; k < kMetaPerThread; ++k) {
-      const int64_t i = base + k * 256;
-      if (i >= a.num_tokens) break;
-      int32_t b = -1, pos = -1, slot = -1;
-      if (i < total) {
-        b = meta_find(qo, a.seqs, i);
-        const int64_t at = (int64_t)a.seq_lens[b] - meta_new(a, b) + (i - qo[b]);
-        const int32_t pg = at >= 0 ? (int32_t)((uint32_t)at / (uint32_t)a.page_size) : 0;
-        if (at >= 0 && pg < meta_pages(a, b)) {
-          pos = (int32_t)at;
-          const int32_t page = a.tables[(int64_t)b * a.table_stride + pg];
-          if (page >= 0) slot = page * a.page_size + (pos - pg * a.page_size);
-        }
-      }
-      a.batch_indices[i] = b;
-      a.positions[i] = pos;
-      a.slots[i] = slot;
-      a.rope_positions[i] = pos >= 0 ? pos : 0;
+// SCANNED: the prefix sums are in qo_indptr / kv_indptr already.
+template <bool SCANNED>
+__global__ __launch_bounds__(256) void kv_metadata_kernel(KvMetaArgs a) {
+  const int tid = threadIdx.x;
+  const int64_t work = (int64_t)a.seqs * a.pieces;
+  const bool fill = (int64_t)blockIdx.x >= work;
+  const int32_t r = fill ? a.seqs : (int32_t)(blockIdx.x / a.pieces);
+  const int32_t piece = fill ? 0 : (int32_t)(blockIdx.x - (uint32_t)r * a.pieces);
+  int32_t n = 0, pages = 0;
+  if (!fill) {
+    n = meta_new(a, r);
+    pages = meta_pages(a, r);
+    if (piece > 0 && (int64_t)piece * kMetaPiece >= (n > pages ? n : pages)) return;
+  }
+  int64_t q = 0, p = 0;
+  if constexpr (SCANNED) {
+    q = a.qo_indptr[r];
+    p = a.kv_indptr[r];
+  } else {
+    for (int32_t i = tid; i < r; i += 256) {
+      q += meta_new(a, i);
+      p += meta_pages(a, i);
     }
+    meta_block_sum(q, p);
+    if (tid == 0 && piece == 0) {
+      if (!fill) meta_write_request(a, r, q, p);
+      else if ((int64_t)blockIdx.x == work) meta_write_request(a, a.seqs, q, p);
+    }
+  }
+  if (fill) {  // behind the batch
+    const int64_t at = ((int64_t)blockIdx.x - work) * 256 + tid, step = (int64_t)kMetaFill * 256;
+    for (int64_t i = q + at; i < a.num_tokens; i += step) {
+      a.batch_indices[i] = -1;
+      a.positions[i] = -1;
+      a.slots[i] = -1;
+      a.rope_positions[i] = 0;
+    }
+    for (int64_t i = p + at; i < a.num_pages; i += step) a.kv_indices[i] = -1;
     return;
   }
-  const int32_t total = kv[a.seqs];
-#pragma unroll
-  for (int k = 0; k < kMetaPerThread; ++k) {
-    const int64_t i = base + k * 256;
-    if (i >= a.num_pages) break;
-    int32_t page = -1;
-    if (i < total) {
-      const int32_t r = meta_find(kv, a.seqs, i);
-      page = a.tables[(int64_t)r * a.table_stride + (i - kv[r])];
+  const int32_t* const table = a.tables + (int64_t)r * a.table_stride;
+  const int64_t before = (int64_t)a.seq_lens[r] - n;  // position of the first new token
+  const int64_t most = n > pages ? n : pages, stride = (int64_t)a.pieces * kMetaPiece;
+  for (int64_t j0 = (int64_t)piece * kMetaPiece; j0 < most; j0 += stride) {
+#pragma unroll 4
+    for (int k = 0; k < kMetaPiece / 256; ++k) {
+      const int64_t j = j0 + k * 256 + tid;
+      if (j < pages && p + j < a.num_pages) a.kv_indices[p + j] = table[j];
     }
-    a.kv_indices[i] = page;
+    for (int k = 0; k < kMetaPiece / 256; ++k) {
+      const int64_t j = j0 + k * 256 + tid;
+      if (j >= n || q + j >= a.num_tokens) break;
+      const int64_t at = before + j;
+      const int64_t pg = at >= 0 ? (int64_t)((uint32_t)at / (uint32_t)a.page_size) : 0;
+      int32_t pos = -1, slot = -1;
+      if (at >= 0 && pg < pages) {
+        pos = (int32_t)at;
+        const int32_t page = table[pg];
+        if (page >= 0) slot = page * a.page_size + (pos - (int32_t)pg * a.page_size);
+      }
+      a.batch_indices[q + j] = r;
+      a.positions[q + j] = pos;
+      a.slots[q + j] = slot;
+      a.rope_positions[q + j] = pos >= 0 ? pos : 0;
+    }
   }
-}
-
-__global__ __launch_bounds__(256) void kv_metadata_kernel(KvMetaArgs a) {
-  extern __shared__ int32_t meta_lds[];  // two prefix arrays of seqs + 1 entries
-  int32_t* const qo = meta_lds;
-  int32_t* const kv = meta_lds + a.seqs + 1;
-  const bool writer = blockIdx.x == 0;
-  meta_scan(a, [&](int32_t r, int64_t q, int64_t p) {
-    qo[r] = meta_clip(q, a.num_tokens);
-    kv[r] = meta_clip(p, a.num_pages);
-    if (writer) meta_write_request(a, r, q, p);
-  });
-  __syncthreads();
-  meta_lookups(a, qo, kv);
 }
 
 __global__ __launch_bounds__(256) void kv_metadata_scan_kernel(KvMetaArgs a) {
   meta_scan(a, [&](int32_t r, int64_t q, int64_t p) { meta_write_request(a, r, q, p); });
-}
-__global__ __launch_bounds__(256) void kv_metadata_lookup_kernel(KvMetaArgs a) {
-  meta_lookups(a, a.qo_indptr, a.kv_indptr);
 }
 
 }  // namespace sarathi_hip
@@ -204,22 +220,24 @@ extern "C" int sarathi_build_paged_kv_metadata(
   if (num_seqs >= 0x7fffffffLL || num_tokens >= 0x7fffffffLL || num_kv_pages >= 0x7fffffffLL ||
       max_pages_per_seq >= 0x7fffffffLL)
     return SARATHI_ERR_UNSUPPORTED;
-  const int64_t per_group = 256 * kMetaPerThread;
-  const int64_t tok_groups = (num_tokens + per_group - 1) / per_group;
-  const int64_t groups = tok_groups + (num_kv_pages + per_group - 1) / per_group;
+  // pieces of the longest request there can be, while the requests alone are few workgroups
+  const int64_t longest = num_tokens > max_pages_per_seq ? num_tokens : max_pages_per_seq;
+  int64_t pieces = (longest + kMetaPiece - 1) / kMetaPiece;
+  if (pieces > 1024 / (num_seqs + 1)) pieces = 1024 / (num_seqs + 1);
+  if (pieces < 1) pieces = 1;
+  const int64_t groups = num_seqs * pieces + kMetaFill;
+  if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
   KvMetaArgs a{query_lens,    seq_lens,          block_tables,      qo_indptr,
                kv_indptr,     kv_indices,        kv_last_page_len,  batch_indices,
                positions,     slot_mapping,      rope_positions,    table_stride,
                (int32_t)num_seqs, (int32_t)max_pages_per_seq, (int32_t)page_size,
-               num_tokens,    num_kv_pages,      (uint32_t)tok_groups};
+               num_tokens,    num_kv_pages,      (uint32_t)pieces};
   hipStream_t st = (hipStream_t)stream;
-  if (num_seqs <= kMetaLdsSeqs) {
-    hipLaunchKernelGGL(kv_metadata_kernel, dim3((unsigned)(groups > 0 ? groups : 1)), dim3(256),
-                       (unsigned)(2 * (num_seqs + 1) * sizeof(int32_t)), st, a);
+  if (num_seqs <= kMetaOneLaunch) {
+    hipLaunchKernelGGL((kv_metadata_kernel<false>), dim3((unsigned)groups), dim3(256), 0, st, a);
     return launch_status();
   }
   hipLaunchKernelGGL(kv_metadata_scan_kernel, dim3(1), dim3(256), 0, st, a);
-  if (groups > 0)
-    hipLaunchKernelGGL(kv_metadata_lookup_kernel, dim3((unsigned)groups), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((kv_metadata_kernel<true>), dim3((unsigned)groups), dim3(256), 0, st, a);
   return launch_status();
 }
