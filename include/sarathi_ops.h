@@ -310,7 +310,8 @@ int sarathi_moe_sum(void* out, const void* input, int64_t num_tokens, int64_t to
  * sarathi_append_paged_kv_cache replaces append_paged_kv_cache(..., kv_layout="NHD")
  * (flashinfer_attention_wrapper.py:262-273): token i's key and value rows are copied to entry
  * positions[i] % page_size of page kv_indices[kv_indptr[batch_indices[i]] + positions[i] /
- * page_size].  Indices are not range-checked.
+ * page_size].  A token whose position, request or slot is negative goes nowhere (its cache stores
+ * are dropped: the padding of a captured batch); otherwise indices are not range-checked.
  *
  * sarathi_get_kv_slot_mapping (new) resolves that lookup once per batch:
  * slot_mapping[i] = page * page_size + entry.  The page table of a batch is the same for every
@@ -394,7 +395,7 @@ int sarathi_build_paged_kv_metadata(const int32_t* query_lens, const int32_t* se
  * kv_indices[kv_indptr[r] .. kv_indptr[r + 1]); the cache geometry is that of
  * sarathi_append_paged_kv_cache.  Query head h uses key head h / (num_heads / num_kv_heads).
  * With n new tokens and s keys, new token j has index x = s - n + j and sees keys i <= x (causal),
- * of these i >= x - window_left (window_left >= 0), scaled by sm_scale:
+ * of these i >= x - window_left (window_left >= 0), scaled by sm_scale (positive and finite):
  *   lse = log sum_i exp(sm_scale <q, k_i>),   out = sum_i exp(sm_scale <q, k_i> - lse) v_i.
  * A token that sees no key gets out = 0, lse = -inf.  lse (float [num_tokens, num_heads], natural
  * logarithm) may be NULL.  Rows of out and lse outside [qo_indptr[0], qo_indptr[num_seqs]) are left

@@ -57,8 +57,9 @@ __global__ __launch_bounds__(64) void kv_append_tok_kernel(
 #pragma unroll
   for (int t = 0; t < TPW; ++t) {
     const int64_t e = kv_entry_resolve<SLOTS>(d, keys[t]);
-    const rsrc_t dk = make_rsrc(reinterpret_cast<char*>(d.k_cache) + e, recs[t]);
-    const rsrc_t dv = make_rsrc(reinterpret_cast<char*>(d.v_cache) + e, recs[t]);
+    const uint32_t rec = e < 0 ? 0u : recs[t];  // nowhere to go: stores dropped
+    const rsrc_t dk = make_rsrc(reinterpret_cast<char*>(d.k_cache) + e, rec);
+    const rsrc_t dv = make_rsrc(reinterpret_cast<char*>(d.v_cache) + e, rec);
 #pragma unroll
     for (int p = 0; p < PPL; ++p) buf_store16<kKvStore>(dk, off + p * 1024u, kk[t][p]);
 #pragma unroll
@@ -105,8 +106,10 @@ __global__ __launch_bounds__(64) void kv_append_seg_kernel(
   const char* src = reinterpret_cast<const char*>(is_k ? key : value) +
                     tok * (is_k ? k_stride_bytes : v_stride_bytes);
   const u32x4 v = buf_load16<kStreamLoad>(make_rsrc(src, row_bytes), off);
-  char* dst = reinterpret_cast<char*>(is_k ? d.k_cache : d.v_cache) + kv_entry_offset(d, tok);
-  buf_store16<kKvStore>(make_rsrc(dst, row_bytes), off, v);  // pieces past the row are dropped
+  const int64_t e = kv_entry_offset(d, tok);
+  char* dst = reinterpret_cast<char*>(is_k ? d.k_cache : d.v_cache) + e;
+  // pieces past the row are dropped, and all of a token that goes nowhere
+  buf_store16<kKvStore>(make_rsrc(dst, e < 0 ? 0u : row_bytes), off, v);
 }
 
 // Any alignment: one workgroup per token, 2-byte units (every supported dtype is a multiple).
@@ -115,6 +118,7 @@ __global__ __launch_bounds__(256) void kv_append_generic_kernel(
     int64_t v_stride_bytes, uint32_t row_bytes, KvDest d) {
   const int64_t tok = blockIdx.x;
   const int64_t e = kv_entry_offset(d, tok);
+  if (e < 0) return;
   const uint16_t* ks =
       reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(key) + tok * k_stride_bytes);
   const uint16_t* vs = reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(value) +
@@ -161,6 +165,10 @@ __global__ __launch_bounds__(256) void kv_slot_mapping_kernel(
     int32_t* __restrict__ slot_mapping, int64_t nnz, int32_t page_size) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= nnz) return;
+  if ((batch_indices[i] | positions[i]) < 0) {  // goes nowhere: see kv_dest.h
+    slot_mapping[i] = -1;
+    return;
+  }
   const uint32_t pos = (uint32_t)positions[i];
   const uint32_t pg = pos / (uint32_t)page_size;
   const int32_t page = kv_indices[(int64_t)kv_indptr[batch_indices[i]] + pg];

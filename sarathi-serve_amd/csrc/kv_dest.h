@@ -65,14 +65,18 @@ SK_DEV KvEntryKey kv_entry_key(const KvDest& d, int64_t tok) {
   return k;
 }
 // SLOTS: whether k.a is a slot (known at compile time where a kernel is specialised on it).
+// Returns -1 for a token that goes nowhere: a negative slot, request or position (the rows behind
+// the last sequence of a padded batch).  Its stores are dropped; no table is looked up for it.
 template <bool SLOTS>
 SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
   if (SLOTS) {
+    if (k.a < 0) return -1;
     const uint32_t slot = (uint32_t)k.a;
     const uint32_t page = slot / (uint32_t)d.page_size;
     const uint32_t entry = slot - page * (uint32_t)d.page_size;
     return (int64_t)page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
   }
+  if ((k.a | k.b) < 0) return -1;
   const uint32_t pos = (uint32_t)k.b;
   const uint32_t pg = pos / (uint32_t)d.page_size;
   const uint32_t entry = pos - pg * (uint32_t)d.page_size;

@@ -402,6 +402,8 @@ extern "C" int sarathi_paged_attention(
   if (!attn_sizes_ok(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads, head_size,
                      page_size) || num_pages < 0)
     return SARATHI_ERR_INVALID_ARG;
+  // maxima are taken before scaling, and masked scores are -inf: the scale is positive and finite
+  if (!(sm_scale > 0.f) || !(sm_scale * kLog2e < INFINITY)) return SARATHI_ERR_INVALID_ARG;
   const int64_t row = (int64_t)num_heads * head_size, kv_row = (int64_t)num_kv_heads * head_size;
   if ((num_tokens > 1 && (query_stride < row || out_stride < row)) || entry_stride < kv_row ||
       page_stride < 0)

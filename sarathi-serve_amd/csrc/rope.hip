@@ -315,8 +315,9 @@ SK_DEV void rope_wave(const int64_t* __restrict__ positions, void* a,
       const bool is_k = seg_in_a == a_is_key;
       in_place = !is_k || write_key != 0 || !appended;
       if (is_k && appended) {  // uniform
-        const rsrc_t rkc = make_rsrc(reinterpret_cast<char*>(d->k_cache) + entry, kv_row_bytes);
-        const rsrc_t rvc = make_rsrc(reinterpret_cast<char*>(d->v_cache) + entry, kv_row_bytes);
+        const uint32_t rec = entry < 0 ? 0u : kv_row_bytes;  // nowhere to go: stores dropped
+        const rsrc_t rkc = make_rsrc(reinterpret_cast<char*>(d->k_cache) + entry, rec);
+        const rsrc_t rvc = make_rsrc(reinterpret_cast<char*>(d->v_cache) + entry, rec);
         buf_store16<KSP>(rkc, koff[j], xr[j]);
         if constexpr (NEOX) buf_store16<KSP>(rkc, kyoff(j), yr[j]);
         buf_store16<KSP>(rvc, koff[j], vx[j]);
@@ -638,6 +639,7 @@ __global__ __launch_bounds__(256) void rope_append_generic_kernel(RopeArgs a, co
   const int64_t crow = a.positions[tok] * a.rot_dim;
   const bool appended = tok < d.nnz;
   const int64_t e = appended ? kv_entry_offset(d, tok) : 0;
+  const bool stored = appended && e >= 0;
   void* kc = reinterpret_cast<char*>(d.k_cache) + e;
   void* vc = reinterpret_cast<char*>(d.v_cache) + e;
   const int nq = a.num_heads * embed;
@@ -657,12 +659,12 @@ __global__ __launch_bounds__(256) void rope_append_generic_kernel(RopeArgs a, co
       store_elem<DT>(arr, hb + xo, ox);
       store_elem<DT>(arr, hb + yo, oy);
     }
-    if (!is_q && appended) {
+    if (!is_q && stored) {
       store_elem<DT>(kc, hl + xo, ox);
       store_elem<DT>(kc, hl + yo, oy);
     }
   }
-  if (!appended) return;
+  if (!stored) return;
   // the un-rotated tail of every k head, then the v row
   const int tail = a.head_size - a.rot_dim;
   for (int i = threadIdx.x; i < a.num_kv_heads * tail; i += 256) {

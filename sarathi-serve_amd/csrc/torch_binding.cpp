@@ -509,6 +509,8 @@ std::vector<torch::Tensor> paged_attention(
   TORCH_CHECK(qo_indptr.numel() == seqs + 1 && kv_indptr.numel() == seqs + 1, op,
               ": expected qo_indptr and kv_indptr [n+1], kv_last_page_len [n]");
   TORCH_CHECK(max_query_len >= 0, op, ": max_query_len must not be negative");
+  const double scale = sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt((double)g.head_size);
+  TORCH_CHECK(scale > 0 && std::isfinite((float)scale), op, ": sm_scale must be positive and finite");
   LaunchScope scope(query);
   torch::Tensor out;
   if (out_or_none.has_value()) {
@@ -532,7 +534,6 @@ std::vector<torch::Tensor> paged_attention(
       (int)g.page_size, max_query_len);
   torch::Tensor workspace;
   if (ws > 0) workspace = torch::empty({ws}, query.options().dtype(torch::kUInt8));
-  const double scale = sm_scale.has_value() ? *sm_scale : 1.0 / std::sqrt((double)g.head_size);
   raise_on(sarathi_paged_attention(
                query.data_ptr(), k_ptr, v_ptr, out.data_ptr(), lse, qo_indptr.data_ptr<int32_t>(),
                kv_indptr.data_ptr<int32_t>(), kv_indices.data_ptr<int32_t>(),

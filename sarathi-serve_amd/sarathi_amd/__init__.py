@@ -16,10 +16,13 @@ signatures (the reference builds them as four pybind11 modules, setup.py:95-136)
 
 ``kv_cache_ops`` adds the paged KV-cache append that follows the rotary embedding on the
 reference's attention path (flashinfer's get_seq_lens / get_batch_indices_positions /
-append_paged_kv_cache signatures) and its fusion with rotary_embedding.
+append_paged_kv_cache signatures) and its fusion with rotary_embedding, and what reads the cache:
+the index vectors of a batch built on the GPU, attention of a hybrid batch over its pages and the
+join of attention states.
 
-All ops return None, write through out-parameters or in place, and launch
-asynchronously on torch's current stream.  There is no CPU or PyTorch fallback:
+The ops that the reference has return None and write through out-parameters or in place; those of
+``kv_cache_ops`` that make new tensors return them.  All launch asynchronously on torch's current
+stream.  There is no CPU or PyTorch fallback:
 importing this package raises ImportError when the compiled HIP extension is
 missing.  ``sarathi_amd.layers`` holds counterparts of the reference's Python
 layer classes that call these ops.

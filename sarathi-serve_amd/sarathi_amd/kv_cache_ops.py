@@ -136,7 +136,7 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: 
     buffer), bfloat16 or float16; the tokens of request r are ``[qo_indptr[r], qo_indptr[r + 1])``
     and are the last ones of its sequence, whose keys the four kv vectors describe as for the append.
     With ``causal`` a token sees the keys up to its own, with ``window_left >= 0`` only that many
-    before it.  ``sm_scale`` defaults to ``head_size ** -0.5``.  ``max_query_len``, where the caller
+    before it.  ``sm_scale``, positive, defaults to ``head_size ** -0.5``.  ``max_query_len``, where the caller
     knows an upper bound of the requests' new tokens, picks the kernel (1: a pure decode batch).
 
     Returns ``out`` (shaped like ``query``), with ``return_lse`` also the natural-log sums

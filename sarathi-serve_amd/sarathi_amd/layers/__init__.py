@@ -7,7 +7,8 @@ from .fused_moe import (PackedExpertWeights, fused_experts, fused_moe, get_defau
                         get_moe_configs, invoke_fused_moe_kernel, pack_expert_weights,
                         try_get_optimal_moe_config)
 from .fused_moe_layer import FusedMoE
-from .kv_append import AppendMetadata, SequenceSlice, build_append_metadata
+from .kv_append import (AppendMetadata, SequenceSlice, build_append_metadata,
+                        build_append_metadata_on_device)
 from .moe_routing import (balance_blocks, fused_topk, fused_topk_and_align, grouped_topk,
                           moe_align_block_size)
 from .norm import RMSNorm
@@ -21,4 +22,5 @@ __all__ = ["RMSNorm", "SiluAndMul", "NewGELU", "FastGELU", "get_act_fn", "Rotary
            "invoke_fused_moe_kernel", "fused_experts", "fused_moe", "FusedMoE", "get_default_config",
            "get_moe_configs", "try_get_optimal_moe_config", "pack_expert_weights",
            "PackedExpertWeights", "SequenceSlice", "AppendMetadata", "build_append_metadata",
+           "build_append_metadata_on_device",
            "op_timer", "set_op_timer_factory", "balance_blocks"]

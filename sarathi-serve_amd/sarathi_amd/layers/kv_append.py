@@ -1,6 +1,8 @@
-"""Host-side index bookkeeping for the paged KV-cache append of a hybrid batch (reference:
-FlashinferAttentionWrapper.begin_forward,
-sarathi/model_executor/attention/flashinfer_attention_wrapper.py:84-229).
+"""Index bookkeeping of a hybrid batch for the paged KV-cache append and the attention over the cache
+(reference: FlashinferAttentionWrapper.begin_forward,
+sarathi/model_executor/attention/flashinfer_attention_wrapper.py:84-229), from host lists
+(``build_append_metadata``) or from lengths and page tables that live on the GPU
+(``build_append_metadata_on_device``).
 
 A batch is prefill chunks first, then one decode token per running request.  For every request
 the page table prefix in use, the fill of its last page and the start of its tokens in the
@@ -12,7 +14,7 @@ model: it is computed once here and every append of the batch (``AppendMetadata.
 index load per token instead of three dependent ones.
 """
 from dataclasses import dataclass
-from typing import List, Sequence
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -41,6 +43,8 @@ class AppendMetadata:
     slot_mapping: torch.Tensor              # [num_total_tokens] page * block_size + entry
     num_prefill_tokens: int
     num_total_tokens: int
+    max_query_len: Optional[int] = None             # most new tokens of a request, where known
+    rope_positions: Optional[torch.Tensor] = None   # append_positions as the rotary embedding's int64
 
     def append(self, key: torch.Tensor, value: torch.Tensor, kv_cache, kv_layout: str = "NHD") -> None:
         """The append of FlashinferAttentionWrapper.forward
@@ -63,6 +67,32 @@ class AppendMetadata:
             write_key, kv_layout, slot_mapping=self.slot_mapping)
 
 
+    def attention(self, query: torch.Tensor, kv_cache, softmax_scale: Optional[float] = None,
+                  window_left: int = -1, out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                  kv_layout: str = "NHD"):
+        """Causal attention of this batch's tokens over their sequences, after the append: the prefill
+        and the decode wrapper of FlashinferAttentionWrapper.forward
+        (sarathi/model_executor/attention/flashinfer_attention_wrapper.py:275-304) in one call."""
+        return kv_cache_ops.paged_attention(
+            query, kv_cache, self.append_qo_indptr, self.append_kv_page_indptr, self.append_kv_page_indices,
+            self.append_kv_last_page_len, sm_scale=softmax_scale, causal=True, window_left=window_left,
+            max_query_len=self.max_query_len, out=out, return_lse=return_lse, kv_layout=kv_layout)
+
+
+def build_append_metadata_on_device(query_lens: torch.Tensor, seq_lens: torch.Tensor,
+                                    block_tables: torch.Tensor, block_size: int, num_total_tokens: int,
+                                    num_kv_pages: Optional[int] = None, num_prefill_tokens: int = 0,
+                                    max_query_len: Optional[int] = None) -> AppendMetadata:
+    """``build_append_metadata`` for a batch whose lengths and page tables are on the GPU: one kernel,
+    no copy, no synchronisation, fit for capture (see ``kv_cache_ops.build_paged_kv_metadata`` for the
+    arguments and for what padding is filled with).  The order of the requests is the caller's."""
+    m = kv_cache_ops.build_paged_kv_metadata(query_lens, seq_lens, block_tables, block_size,
+                                             num_total_tokens, num_kv_pages)
+    return AppendMetadata(m.qo_indptr, m.kv_indices, m.kv_indptr, m.kv_last_page_len, m.batch_indices,
+                          m.positions, m.slot_mapping, num_prefill_tokens, num_total_tokens,
+                          max_query_len, m.rope_positions)
+
+
 def build_append_metadata(seqs: Sequence[SequenceSlice], block_size: int,
                           device: torch.device) -> AppendMetadata:
     qo_indptr: List[int] = [0]
@@ -70,6 +100,7 @@ def build_append_metadata(seqs: Sequence[SequenceSlice], block_size: int,
     page_indptr: List[int] = [0]
     last_page_len: List[int] = []
     num_prefill_tokens = 0
+    max_query_len = 0
     # prompts first, then decodes, each group in batch order (flashinfer_attention_wrapper.py:113-168)
     for want_prompt in (True, False):
         for s in seqs:
@@ -80,6 +111,7 @@ def build_append_metadata(seqs: Sequence[SequenceSlice], block_size: int,
             if len(s.block_table) < blocks:
                 raise ValueError("block_table holds %d pages, %d tokens need %d"
                                  % (len(s.block_table), s.total_len, blocks))
+            max_query_len = max(max_query_len, new)
             qo_indptr.append(qo_indptr[-1] + new)
             page_indices.extend(s.block_table[:blocks])
             page_indptr.append(page_indptr[-1] + blocks)
@@ -99,4 +131,4 @@ def build_append_metadata(seqs: Sequence[SequenceSlice], block_size: int,
     slot_mapping = kv_cache_ops.get_kv_slot_mapping(batch_indices, positions, m_idx, m_indptr,
                                                     block_size)
     return AppendMetadata(m_qo, m_idx, m_indptr, m_last, batch_indices, positions, slot_mapping,
-                          num_prefill_tokens, num_total_tokens)
+                          num_prefill_tokens, num_total_tokens, max_query_len or None)
