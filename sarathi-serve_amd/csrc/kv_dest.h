@@ -70,11 +70,11 @@ SK_DEV KvEntryKey kv_entry_key(const KvDest& d, int64_t tok) {
 template <bool SLOTS>
 SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
   if (SLOTS) {
-    if (k.a < 0) return -1;
     const uint32_t slot = (uint32_t)k.a;
     const uint32_t page = slot / (uint32_t)d.page_size;
     const uint32_t entry = slot - page * (uint32_t)d.page_size;
-    return (int64_t)page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
+    const int64_t at = (int64_t)page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
+    return k.a < 0 ? -1 : at;  // a select: no branch
   }
   if ((k.a | k.b) < 0) return -1;
   const uint32_t pos = (uint32_t)k.b;

@@ -33,8 +33,10 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
   const uint32_t head = vec / per_head;
   if (head >= (uint32_t)a.heads) return;
   const float* lse = a.lse + tok * a.lse_token + head;
-  const char* v = reinterpret_cast<const char*>(a.v) + (tok * a.v_token + (int64_t)vec * E) * ElemBytes<DT>::value;
+  // rows of a token: the same for the workgroup, so scalar buffer resources
+  const char* v = reinterpret_cast<const char*>(a.v) + tok * a.v_token * ElemBytes<DT>::value;
   const int64_t step = a.v_state * ElemBytes<DT>::value;
+  const uint32_t row_bytes = (uint32_t)a.heads * (uint32_t)a.head_size * ElemBytes<DT>::value;
   float top = -INFINITY, l = 0.f;
   Vec<DT> acc;
 #pragma unroll
@@ -45,7 +47,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
 #pragma unroll
     for (int s = 0; s < N; ++s) z[s] = lse[s * a.lse_state];
 #pragma unroll
-    for (int s = 0; s < N; ++s) raw[s] = *reinterpret_cast<const u32x4*>(v + s * step);
+    for (int s = 0; s < N; ++s) raw[s] = buf_load16<kStreamLoad>(make_rsrc(v + s * step, row_bytes), vec * 16u);
     __builtin_amdgcn_sched_barrier(0);  // every load is issued before anything waits
 #pragma unroll
     for (int s = 0; s < N; ++s) top = fmaxf(top, z[s]);
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
       const float w = __builtin_amdgcn_exp2f((z - ref) * kLog2e);
       l += w;
       Vec<DT> x;
-      x.unpack(*reinterpret_cast<const u32x4*>(v + s * step));
+      x.unpack(buf_load16<kStreamLoad>(make_rsrc(v + s * step, row_bytes), vec * 16u));
 #pragma unroll
       for (int i = 0; i < E; ++i) acc.f[i] = fmaf(z == -INFINITY ? 0.f : x.f[i], w, acc.f[i]);
     }
@@ -76,8 +78,9 @@ __global__ __launch_bounds__(256) void merge_states_kernel(MergeArgs a) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc.f[i] *= inv;
-  *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(a.out) +
-                            (tok * a.out_token + (int64_t)vec * E) * ElemBytes<DT>::value) = acc.pack();
+  buf_store16<kStreamStore>(
+      make_rsrc(reinterpret_cast<char*>(a.out) + tok * a.out_token * ElemBytes<DT>::value, row_bytes),
+      vec * 16u, acc.pack());
   if (a.out_lse && vec == head * per_head)
     a.out_lse[tok * a.out_lse_token + head] = l == 0.f ? -INFINITY : top + logf(l);
 }
@@ -139,7 +142,7 @@ extern "C" int sarathi_merge_attention_states(const void* v, const float* lse, v
                          (out_lse && out_lse_token_stride < num_heads)))
     return SARATHI_ERR_INVALID_ARG;
   if (dtype != kF32 && dtype != kF16 && dtype != kBF16) return SARATHI_ERR_UNSUPPORTED;
-  if (num_states > 0x7fffffffLL || row > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
+  if (num_states > 0x7fffffffLL || row > 0x1fffffffLL) return SARATHI_ERR_UNSUPPORTED;
   if (num_tokens == 0) return SARATHI_OK;
   if (!v || !lse || !out) return SARATHI_ERR_INVALID_ARG;
   MergeArgs a{v, lse, out, out_lse, v_state_stride, v_token_stride, lse_state_stride,
