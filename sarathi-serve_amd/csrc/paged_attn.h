@@ -411,8 +411,11 @@ template <int DP, bool PAD, bool PAGE16, int IDS, bool ONCE> struct ShareLoader 
   SK_DEV int32_t clamp_key(int32_t t) const { return t < first ? first : t < end ? t : end - 1; }
   // the share at key t, or the nearest one that holds a key
   SK_DEV int32_t base(int32_t t) const { return clamp_i32(t, first & ~15, (end - 1) & ~15); }
+  // its page number, through the scalar cache: as a vector load its wait would be one for every load
+  // into LDS that is in flight (nothing writes page numbers while a kernel runs)
   SK_DEV int32_t page(int32_t t) const {
-    return PAGE16 ? a.kv_indices[x.kv0 + attn_page_of(a, base(t))] : 0;
+    if constexpr (!PAGE16) return 0;
+    return ((const __attribute__((address_space(4))) int32_t*)a.kv_indices)[x.kv0 + attn_page_of(a, base(t))];
   }
   SK_DEV void load_ids(int32_t t, int32_t n) const {
     if constexpr (!PAGE16) {
