@@ -113,15 +113,21 @@ struct AttnItem {
   int32_t tile;      // tile of its rows
   int32_t part, parts, part_len;
   int32_t state_row; // first state row of this tile and part (key head 0)
+  AttnSeq seq;
 };
 
-SK_DEV uint64_t wave_scan_u64(uint64_t v, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
-  return v;
+// Inclusive sum over the lanes up to one's own: sixteen lanes by row shifts, then the row totals are
+// broadcast to the rows behind.
+template <int CTRL, int ROWS> SK_DEV uint32_t dpp_scan_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+SK_DEV uint32_t wave_scan(uint32_t v) {
+  v = dpp_scan_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_scan_add<0x112, 0xf>(v);
+  v = dpp_scan_add<0x114, 0xf>(v);
+  v = dpp_scan_add<0x118, 0xf>(v);
+  v = dpp_scan_add<0x142, 0xa>(v);  // lane 15 of a row to the next: rows 1 and 3
+  return dpp_scan_add<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
 }
 
 // Most keys that a tile of the request spans, counted from a multiple of 64 where a window cuts the
@@ -137,12 +143,13 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
 // GPU once allows but no longer than kPartKeys (below, its start and the way of its state to memory
 // and back weigh in), unless that made more than `target` items; it is at least min_part keys and a
 // multiple of 64.  When nothing is cut the first is left out.  The
-// workgroup with `map` set leaves the state rows for the kernel that joins the parts.  Sums of the
-// two classes share a word: tiles times keys stay far below 2^40 each in units of 64 keys, items
-// below 2^31.
+// workgroup with `map` set leaves the state rows for the kernel that joins the parts.  The work is
+// summed in 32-bit floats (it only chooses a length, the same in every workgroup; rounded up by more
+// than their error, so that the items stay within what the launch has workgroups for).
 template <int WAVES>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
-  __shared__ uint64_t sums[2][WAVES];
+  __shared__ float work_sums[2][WAVES];
+  __shared__ uint32_t sums[2][WAVES];
   __shared__ AttnItem found;
   constexpr int NT = WAVES * 64, KEEP = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -150,7 +157,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   const int64_t first = (int64_t)tid * run;
   const int32_t r0 = first < a.seqs ? (int32_t)first : a.seqs;
   const int32_t r1 = first + run < a.seqs ? (int32_t)(first + run) : a.seqs;
-  struct Load { int32_t tiles, keys; bool tiled; };
+  struct Load { int32_t tiles, keys; bool tiled; AttnSeq seq; };
   auto look = [&](int32_t r) {
     const AttnSeq x = attn_seq(a, r);
     const int64_t rows = (int64_t)x.n * a.group;
@@ -159,12 +166,13 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     const int32_t lg = v.tiled ? a.tile.rows_log2 : a.few.rows_log2;
     v.tiles = (int32_t)((rows + ((int64_t)1 << lg) - 1) >> lg);
     v.keys = attn_keys(a, x);
+    v.seq = x;
     return v;
   };
   Load kept[KEEP];  // the first requests of this thread are looked at once
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
-    kept[i] = {0, 0, false};
+    kept[i] = {0, 0, false, {0, 0, 0, 0}};
     if (r0 + i < r1) kept[i] = look(r0 + i);
   }
   auto each = [&](auto f) {
@@ -176,58 +184,60 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   if (tid == 0) found.r = -1;
   int32_t few_len = 0x7fffffff, tile_len = 0x7fffffff;
   if (a.few.target > 0 || a.tile.target > 0) {
-    uint64_t few = 0, tile = 0;
+    float few = 0.f, tile = 0.f;
     each([&](int32_t, const Load& v) {
-      (v.tiled ? tile : few) += (uint64_t)v.tiles * (uint32_t)((v.keys + 63) >> 6);
+      (v.tiled ? tile : few) += (float)v.tiles * (float)((v.keys + 63) >> 6);
     });
-    few = wave_scan_u64(few, lane);
-    tile = wave_scan_u64(tile, lane);
-    if (lane == 63) {
-      sums[0][wave] = few;
-      sums[1][wave] = tile;
+    few = wave64_sum(few);
+    tile = wave64_sum(tile);
+    if (lane == 0) {
+      work_sums[0][wave] = few;
+      work_sums[1][wave] = tile;
     }
     __syncthreads();
-    few = tile = 0;
+    few = tile = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      few += sums[0][w];
-      tile += sums[1][w];
+      few += work_sums[0][w];
+      tile += work_sums[1][w];
     }
-    auto length = [](uint64_t work, const AttnClass& c) {
+    auto length = [](float work, const AttnClass& c) {
       if (c.target <= 0) return 0x7fffffff;
-      uint64_t len = (work + (uint32_t)c.fill - 1) / (uint32_t)c.fill;
-      if (len > kPartKeys / 64) len = kPartKeys / 64;
-      const uint64_t least = (work + (uint32_t)c.target - 1) / (uint32_t)c.target;
-      if (len < least) len = least;
-      const int32_t keys = len > 0xffffffull ? 0x3fffffc0 : (int32_t)len * 64;
+      work *= 1.001f;
+      const float len = fmaxf(fminf(work / (float)c.fill, kPartKeys / 64), work / (float)c.target);
+      const int32_t keys = len > 1.6e7f ? 0x3fffffc0 : (int32_t)ceilf(len) * 64;
       return keys > c.min_part ? keys : c.min_part;
     };
     few_len = length(few, a.few);
     tile_len = length(tile, a.tile);
-    __syncthreads();  // sums[] is written again below
   }
   auto parts_of = [&](const Load& v) {
     const int32_t len = v.tiled ? tile_len : few_len;
     return v.keys <= len ? 1 : (v.keys - 1) / len + 1;
   };
-  // chunks' items in the upper half, those of few rows in the lower
-  uint64_t mine = 0;
-  each([&](int32_t, const Load& v) {
-    mine += (uint64_t)(uint32_t)(v.tiles * parts_of(v)) << (v.tiled ? 32 : 0);
-  });
-  const uint64_t incl = wave_scan_u64(mine, lane);
-  if (lane == 63) sums[0][wave] = incl;
+  uint32_t my_few = 0, my_tile = 0;
+  each([&](int32_t, const Load& v) { (v.tiled ? my_tile : my_few) += (uint32_t)(v.tiles * parts_of(v)); });
+  uint32_t few_at = wave_scan(my_few), tile_at = wave_scan(my_tile);
+  if (lane == 63) {
+    sums[0][wave] = few_at;
+    sums[1][wave] = tile_at;
+  }
+  few_at -= my_few;
+  tile_at -= my_tile;
   __syncthreads();
-  uint64_t at = incl - mine, all = 0;
+  uint32_t few_items = 0, tile_items = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) at += sums[0][w];
-    all += sums[0][w];
+    if (w < wave) {
+      few_at += sums[0][w];
+      tile_at += sums[1][w];
+    }
+    few_items += sums[0][w];
+    tile_items += sums[1][w];
   }
   // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
   // are at work all the time; the last quarter of the few ones evens out the end.  Batch of 2304
   // tokens: 876 us, 945 with all tiles first.
-  const uint32_t tile_items = (uint32_t)(all >> 32), few_items = (uint32_t)all;
   const uint32_t mixed = tile_items + (uint32_t)((uint64_t)few_items * 3 / 4);
   uint32_t tiles_before = tile_items;
   bool tiled = false;
@@ -236,7 +246,6 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     tiled = (uint32_t)(((uint64_t)(want + 1) * tile_items + mixed - 1) / mixed) > tiles_before;
   }
   const uint32_t in_class = tiled ? tiles_before : want - tiles_before;
-  uint32_t tile_at = (uint32_t)(at >> 32), few_at = (uint32_t)at;
   int32_t cut = 0;
   each([&](int32_t r, const Load& v) {
     const int32_t parts = parts_of(v);
@@ -254,7 +263,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       // a chunk's last tokens have the most keys: its last tile comes first
       const int32_t tile = v.tiled ? v.tiles - 1 - in / parts : in / parts, part = in % parts;
       found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
-               state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2)};
+               state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2), v.seq};
     }
     mine_at += cnt;
   });
@@ -271,6 +280,10 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   it.parts = __builtin_amdgcn_readfirstlane(found.parts);
   it.part_len = __builtin_amdgcn_readfirstlane(found.part_len);
   it.state_row = __builtin_amdgcn_readfirstlane(found.state_row);
+  it.seq.q0 = __builtin_amdgcn_readfirstlane(found.seq.q0);
+  it.seq.n = __builtin_amdgcn_readfirstlane(found.seq.n);
+  it.seq.kv0 = __builtin_amdgcn_readfirstlane(found.seq.kv0);
+  it.seq.s = __builtin_amdgcn_readfirstlane(found.seq.s);
   return it;
 }
 

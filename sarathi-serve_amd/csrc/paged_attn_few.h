@@ -39,7 +39,7 @@ SK_DEV void few_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, lds
   constexpr int kOps = 2 * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads a wave issues per block
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const AttnSeq x = attn_seq(a, it.r);
+  const AttnSeq x = it.seq;
   const int32_t rows_all = x.n * a.group, row0 = it.tile * ROWS;
   const int32_t rows = rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
 

@@ -59,7 +59,7 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int share = wave & 3;
-  const AttnSeq x = attn_seq(a, it.r);
+  const AttnSeq x = it.seq;
   const int32_t rows_all = x.n * a.group;
   const int32_t row0 = it.tile * ROWS;
   const int32_t rows = rows_all - row0 < ROWS ? rows_all - row0 : ROWS;
