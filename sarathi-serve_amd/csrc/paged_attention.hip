@@ -332,6 +332,7 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
     return target < most ? target : most;
   };
   few_target = bound(few_target, p.few, few_tiles);
+  if (capacity <= kCutKeys + 128) few_target = 0;
   if (chunk_target > 0) chunk_target = bound(chunk_target, p.tile, chunk_tiles);
   // every request is of one class: the tiles that are there at most
   int64_t tiles = p.tile.rows_log2 < 0 ? few_tiles : (all_rows >> p.tile.rows_log2) + seqs;

@@ -106,6 +106,7 @@ SK_DEV int64_t attn_entry(const PagedAttnArgs& a, const AttnSeq& x, int32_t pos)
 // ---- work items ------------------------------------------------------------------------------
 
 constexpr int kPartKeys = 1024;
+constexpr int kCutKeys = 512;
 
 struct AttnItem {
   int32_t r;         // request, -1: none
@@ -142,13 +143,14 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
 // which fix the classes' part lengths, and the numbers of items.  A part is as long as filling the
 // GPU once allows but no longer than kPartKeys (below, its start and the way of its state to memory
 // and back weigh in), unless that made more than `target` items; it is at least min_part keys and a
-// multiple of 64.  When nothing is cut the first is left out.  The
+// multiple of 64.  Where no context is more than kCutKeys longer than that, nothing is cut: a workgroup
+// takes about 5 us for 512 keys, and joining parts as long.  When nothing is cut the first is left out.  The
 // workgroup with `map` set leaves the state rows for the kernel that joins the parts.  The work is
 // summed in 32-bit floats (it only chooses a length, the same in every workgroup; rounded up by more
 // than their error, so that the items stay within what the launch has workgroups for).
 template <int WAVES>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
-  __shared__ float work_sums[2][WAVES];
+  __shared__ float work_sums[2][2][WAVES];
   __shared__ uint32_t sums[2][WAVES];
   __shared__ AttnItem found;
   constexpr int NT = WAVES * 64, KEEP = 2;
@@ -184,32 +186,40 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   if (tid == 0) found.r = -1;
   int32_t few_len = 0x7fffffff, tile_len = 0x7fffffff;
   if (a.few.target > 0 || a.tile.target > 0) {
-    float few = 0.f, tile = 0.f;
+    float few = 0.f, tile = 0.f, few_most = 0.f, tile_most = 0.f;  // keys times tiles; longest
     each([&](int32_t, const Load& v) {
-      (v.tiled ? tile : few) += (float)v.tiles * (float)((v.keys + 63) >> 6);
+      const float blocks = (float)((v.keys + 63) >> 6);
+      (v.tiled ? tile : few) += (float)v.tiles * blocks;
+      float& most = v.tiled ? tile_most : few_most;
+      if (v.tiles > 0) most = fmaxf(most, blocks);
     });
     few = wave64_sum(few);
     tile = wave64_sum(tile);
+    few_most = wave64_max(few_most);
+    tile_most = wave64_max(tile_most);
     if (lane == 0) {
-      work_sums[0][wave] = few;
-      work_sums[1][wave] = tile;
+      work_sums[0][0][wave] = few;
+      work_sums[0][1][wave] = few_most;
+      work_sums[1][0][wave] = tile;
+      work_sums[1][1][wave] = tile_most;
     }
     __syncthreads();
-    few = tile = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      few += work_sums[0][w];
-      tile += work_sums[1][w];
-    }
-    auto length = [](float work, const AttnClass& c) {
+    auto length = [](const float (&sum)[2][WAVES], const AttnClass& c) {
       if (c.target <= 0) return 0x7fffffff;
+      float work = 0.f, most = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        work += sum[0][w];
+        most = fmaxf(most, sum[1][w]);
+      }
       work *= 1.001f;
       const float len = fmaxf(fminf(work / (float)c.fill, kPartKeys / 64), work / (float)c.target);
+      if (most <= len + kCutKeys / 64) return 0x7fffffff;
       const int32_t keys = len > 1.6e7f ? 0x3fffffc0 : (int32_t)ceilf(len) * 64;
       return keys > c.min_part ? keys : c.min_part;
     };
-    few_len = length(few, a.few);
-    tile_len = length(tile, a.tile);
+    few_len = length(work_sums[0], a.few);
+    tile_len = length(work_sums[1], a.tile);
   }
   auto parts_of = [&](const Load& v) {
     const int32_t len = v.tiled ? tile_len : few_len;
