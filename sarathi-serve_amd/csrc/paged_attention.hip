@@ -270,7 +270,6 @@ template <int DT> static int launch_join(const PagedAttnArgs& a, hipStream_t st)
 // head): few rows, and chunks, which are taken in large tiles.  All sizes here are known on the host.
 struct AttnPlan {
   AttnClass few, tile;
-  int waves;           // of a workgroup
   int64_t items;       // at most so many work items per key head, with contexts cut and without
   int64_t uncut_items;
   int64_t map_bytes, ml_bytes, o_bytes;  // of the workspace; 0: nothing is cut
@@ -293,36 +292,36 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   const int64_t units = compute_units();
   const int few_limit = head_size > 128 ? 32 : 64;
   int64_t few_tiles = 0, chunk_tiles = 0, few_target = 0, chunk_target = 0;
-  p.few.fill = 2 * units / kv_heads > 0 ? (int32_t)(2 * units / kv_heads) : 1;
-  p.tile.fill = units / kv_heads > 0 ? (int32_t)(units / kv_heads) : 1;
+  // two workgroups per compute unit
+  p.few.fill = p.tile.fill = 2 * units / kv_heads > 0 ? (int32_t)(2 * units / kv_heads) : 1;
   p.few.rows_log2 = p.tile.rows_log2 = -1;
   if (most_rows <= few_limit || head_size > 128) {
     // all requests in tiles of few rows (max_query_len may be wrong: any number of tiles each)
     const int rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : few_limit;
     p.few.rows_log2 = log2_of(rows);
     p.few.max_rows = 0x7fffffff;
-    p.waves = 4;
     few_tiles = all_rows / rows + seqs;
   } else {
-    // single tokens in one tile each, longer requests in large tiles
-    const int rows = group <= 16 ? 16 : few_limit;
-    p.few.rows_log2 = log2_of(rows);
-    p.few.max_rows = rows;
-    const int big = all_rows / 256 * kv_heads >= units / 2 ? 256 : 128;
-    p.waves = big / 32;
+    // Single tokens in one tile each, longer requests in large tiles; with more than 32 query heads
+    // per key head a single token is a large tile.
+    const int big = 128, rows = group <= 16 ? 16 : group <= 32 ? 32 : 0;
+    if (rows > 0) {
+      p.few.rows_log2 = log2_of(rows);
+      p.few.max_rows = rows;
+      few_tiles = seqs;
+    }
     p.tile.rows_log2 = log2_of(big);
     const int64_t chunks = seqs < all_rows / (rows + 1) ? seqs : all_rows / (rows + 1);
-    few_tiles = seqs;
     chunk_tiles = all_rows / big + chunks;
-    // cut only where the tiles leave a quarter of the compute units idle: a part costs its state's
-    // way to memory and back
-    if (all_rows / big * kv_heads < units * 3 / 4) chunk_target = p.tile.fill;
+    // cut only where the tiles leave a quarter of the GPU idle: a part costs its state's way to
+    // memory and back
+    if (all_rows / big * kv_heads < 2 * units * 3 / 4) chunk_target = p.tile.fill;
     p.tile.min_part = 512;
   }
   if (few_tiles > all_rows) few_tiles = all_rows;
   p.few.min_part = 128;
-  // workgroups of the mixed kernel take twice the waves, and its tiles even out what is left over
-  few_target = (p.tile.rows_log2 < 0 ? 4 : 1) * (int64_t)p.few.fill;
+  // beside chunks, their tiles even out what is left over
+  few_target = p.few.rows_log2 < 0 ? 0 : (p.tile.rows_log2 < 0 ? 4 : 1) * (int64_t)p.few.fill;
   // Cutting yields no more parts than the pages can fill, and where parts are as long as filling the
   // GPU once allows, no more than that takes: the fewer workgroups find nothing to do, the better.
   auto bound = [&](int64_t target, const AttnClass& c, int64_t tiles) {
@@ -331,7 +330,7 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
     if (most > tiles * (capacity / c.min_part)) most = tiles * (capacity / c.min_part);
     return target < most ? target : most;
   };
-  few_target = bound(few_target, p.few, few_tiles);
+  if (few_target > 0) few_target = bound(few_target, p.few, few_tiles);
   if (capacity <= kCutKeys + 128) few_target = 0;
   if (chunk_target > 0) chunk_target = bound(chunk_target, p.tile, chunk_tiles);
   // every request is of one class: the tiles that are there at most
@@ -340,7 +339,8 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   p.uncut_items = tiles;
   p.items = tiles + few_target + chunk_target;
   const int64_t chunk_rows = p.tile.rows_log2 < 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
-  const int64_t state_rows = chunk_rows + (((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
+  const int64_t state_rows =
+      chunk_rows + (p.few.rows_log2 < 0 ? 0 : ((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
   if (few_target + chunk_target == 0 || state_rows >= 0x7fffffffLL) return p;
   p.few.target = (int32_t)few_target;
   p.tile.target = (int32_t)chunk_target;
@@ -357,15 +357,15 @@ using namespace sarathi_hip;
 
 // Heads of up to 128 in batches that may hold chunks take the kernel that does both classes; the
 // others have few rows only.
-static int launch_paged_attn(const PagedAttnArgs& a, int dtype, int waves, bool page16, int64_t groups,
+static int launch_paged_attn(const PagedAttnArgs& a, int dtype, bool page16, int64_t groups,
                              hipStream_t st) {
   if (groups == 0) return SARATHI_OK;
   if (a.tile.rows_log2 < 0) return launch_attn_few(a, dtype, page16, groups, st);
   if (dtype == kBF16)
-    return a.head_size <= 64 ? launch_attn_mixed_bf16_64(a, waves, page16, groups, st)
-                             : launch_attn_mixed_bf16_128(a, waves, page16, groups, st);
-  return a.head_size <= 64 ? launch_attn_mixed_f16_64(a, waves, page16, groups, st)
-                           : launch_attn_mixed_f16_128(a, waves, page16, groups, st);
+    return a.head_size <= 64 ? launch_attn_mixed_bf16_64(a, page16, groups, st)
+                             : launch_attn_mixed_bf16_128(a, page16, groups, st);
+  return a.head_size <= 64 ? launch_attn_mixed_f16_64(a, page16, groups, st)
+                           : launch_attn_mixed_f16_128(a, page16, groups, st);
 }
 
 static bool attn_sizes_ok(int64_t tokens, int64_t seqs, int64_t indices, int heads, int kv_heads,
@@ -478,7 +478,7 @@ extern "C" int sarathi_paged_attention(
   if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
   // offsets inside a share of sixteen keys are 32-bit
   const bool page16 = page_size % 16 == 0 && a.entry_stride < (1 << 26);
-  const int rc = launch_paged_attn(a, dtype, p.waves, page16, groups, st);
+  const int rc = launch_paged_attn(a, dtype, page16, groups, st);
   if (rc != SARATHI_OK || !cut) return rc;
   return dtype == kBF16 ? launch_join<kBF16>(a, st) : launch_join<kF16>(a, st);
 }

@@ -8,21 +8,21 @@
 namespace sarathi_hip {
 
 template <int DT, int DP, int RT, bool PAD, bool PAGE16>
-__global__ __launch_bounds__(256) void paged_attn_few_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(64 * kAttnWaves) void paged_attn_few_kernel(PagedAttnArgs a) {
   extern __shared__ u32x4 few_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
-  const AttnItem it = attn_find_item<4>(a, blockIdx.x / (uint32_t)a.kv_heads,
-                                        a.part_map != nullptr && blockIdx.x == 0);
+  const AttnItem it = attn_find_item(a, blockIdx.x / (uint32_t)a.kv_heads,
+                                     a.part_map != nullptr && blockIdx.x == 0);
   if (it.r < 0) return;
-  few_item<DT, DP, RT, 4, PAD, PAGE16>(a, it, h, (lds_char*)few_lds);
+  few_item<DT, DP, RT, PAD, PAGE16>(a, it, h, (lds_char*)few_lds);
 }
 
 template <int DT, int DP, int RT, bool PAD, bool PAGE16>
 static int launch_few(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
-  constexpr int bytes = few_lds_bytes<DP, RT, 4>();
+  constexpr int bytes = few_lds_bytes<DP, RT>();
   if (!allow_lds<paged_attn_few_kernel<DT, DP, RT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
   hipLaunchKernelGGL((paged_attn_few_kernel<DT, DP, RT, PAD, PAGE16>), dim3((unsigned)groups),
-                     dim3(256), bytes, st, a);
+                     dim3(64 * kAttnWaves), bytes, st, a);
   return launch_status();
 }
 // the exact head size and pages of a multiple of 16 keys have kernels of their own

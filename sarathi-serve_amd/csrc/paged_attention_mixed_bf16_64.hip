@@ -3,8 +3,8 @@
 
 namespace sarathi_hip {
 
-int launch_attn_mixed_bf16_64(const PagedAttnArgs& a, int waves, bool page16, int64_t groups, hipStream_t st) {
-  return launch_mixed<kBF16, 64>(a, waves, page16, groups, st);
+int launch_attn_mixed_bf16_64(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
+  return launch_mixed<kBF16, 64>(a, page16, groups, st);
 }
 
 }  // namespace sarathi_hip

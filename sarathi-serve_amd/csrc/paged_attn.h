@@ -23,6 +23,7 @@
 namespace sarathi_hip {
 
 constexpr int kAttnMaxHead = 256;
+constexpr int kAttnWaves = 4;  // of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -148,8 +149,8 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
 // workgroup with `map` set leaves the state rows for the kernel that joins the parts.  The work is
 // summed in 32-bit floats (it only chooses a length, the same in every workgroup; rounded up by more
 // than their error, so that the items stay within what the launch has workgroups for).
-template <int WAVES>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
+  constexpr int WAVES = kAttnWaves;
   __shared__ float work_sums[2][2][WAVES];
   __shared__ uint32_t sums[2][WAVES];
   __shared__ AttnItem found;

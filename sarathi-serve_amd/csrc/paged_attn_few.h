@@ -26,16 +26,16 @@ template <int DP> struct FewShape : HeadShape<DP> {
   SK_DEV static int swz_v(int row) { return DP == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1; }
 };
 // dynamic LDS: the rings, later the states that half of the waves hand over
-template <int DP, int RT, int WAVES> constexpr int few_lds_bytes() {
-  constexpr int ring = WAVES * FewShape<DP>::kWaveBytes;
-  constexpr int join = WAVES / 2 * 64 * (2 + DP / 16 * 4) * RT * 4;
+template <int DP, int RT> constexpr int few_lds_bytes() {
+  constexpr int ring = kAttnWaves * FewShape<DP>::kWaveBytes;
+  constexpr int join = kAttnWaves / 2 * 64 * (2 + DP / 16 * 4) * RT * 4;
   return ring > join ? ring : join;
 }
 
-template <int DT, int DP, int RT, int WAVES, bool PAD, bool PAGE16>
+template <int DT, int DP, int RT, bool PAD, bool PAGE16>
 SK_DEV void few_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, lds_char* lds) {
   using Sh = FewShape<DP>;
-  constexpr int ROWS = 16 * RT, S = Sh::kStages, KSTEPS = DP / 32, DTILES = DP / 16;
+  constexpr int WAVES = kAttnWaves, ROWS = 16 * RT, S = Sh::kStages, KSTEPS = DP / 32, DTILES = DP / 16;
   constexpr int kOps = 2 * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads a wave issues per block
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);

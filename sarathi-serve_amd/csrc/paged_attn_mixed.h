@@ -1,8 +1,7 @@
-// The attention kernel of hybrid batches: one launch whose work items are the tiles of the chunks,
-// longest first, and then those of the decode tokens.  Chunks are bound by the matrix cores and
-// decodes by memory, so the compute units that are done with their tiles stream keys and values while
-// the others still multiply.  Both kinds of item take a whole compute unit: eight waves, two per SIMD,
-// and about 130 KiB of LDS (four waves where 256-row tiles would be too few to go round).
+// The attention kernel of hybrid batches: one launch whose work items are the tiles of the chunks and
+// those of the decode tokens, in turn.  Chunks are bound by the matrix cores and decodes by memory, so
+// some compute units stream keys and values while the others multiply.  Both kinds of item take half
+// a compute unit: four waves, one per SIMD, and 66 KiB of LDS.
 #pragma once
 
 #include "launch.h"
@@ -12,42 +11,37 @@
 
 namespace sarathi_hip {
 
-template <int DT, int DP, int WAVES, int RT, bool PAD, bool PAGE16>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4)))
+template <int DT, int DP, int RT, bool PAD, bool PAGE16>
+__global__ __launch_bounds__(64 * kAttnWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void paged_attn_mixed_kernel(PagedAttnArgs a) {
   extern __shared__ u32x4 mixed_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
-  const AttnItem it = attn_find_item<WAVES>(a, blockIdx.x / (uint32_t)a.kv_heads,
-                                            a.part_map != nullptr && blockIdx.x == 0);
+  const AttnItem it = attn_find_item(a, blockIdx.x / (uint32_t)a.kv_heads,
+                                     a.part_map != nullptr && blockIdx.x == 0);
   if (it.r < 0) return;
-  if (it.tiled) tile_item<DT, DP, WAVES, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
-  else few_item<DT, DP, RT, WAVES, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
+  if (it.tiled) tile_item<DT, DP, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
+  else few_item<DT, DP, RT, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
 }
 
-template <int DT, int DP, int WAVES, int RT, bool PAD, bool PAGE16>
+template <int DT, int DP, int RT, bool PAD, bool PAGE16>
 static int launch_mixed_form(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
-  constexpr int few = few_lds_bytes<DP, RT, WAVES>(), tile = TileShape<DP>::kBytes;
+  constexpr int few = few_lds_bytes<DP, RT>(), tile = TileShape<DP>::kBytes;
   constexpr int bytes = few > tile ? few : tile;
-  if (!allow_lds<paged_attn_mixed_kernel<DT, DP, WAVES, RT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
-  hipLaunchKernelGGL((paged_attn_mixed_kernel<DT, DP, WAVES, RT, PAD, PAGE16>), dim3((unsigned)groups),
-                     dim3(WAVES * 64), bytes, st, a);
+  if (!allow_lds<paged_attn_mixed_kernel<DT, DP, RT, PAD, PAGE16>>(bytes)) return SARATHI_ERR_LAUNCH;
+  hipLaunchKernelGGL((paged_attn_mixed_kernel<DT, DP, RT, PAD, PAGE16>), dim3((unsigned)groups),
+                     dim3(64 * kAttnWaves), bytes, st, a);
   return launch_status();
 }
-template <int DT, int DP, int WAVES, int RT>
+template <int DT, int DP, int RT>
 static int launch_mixed_rows(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
-  if (!page16) return launch_mixed_form<DT, DP, WAVES, RT, true, false>(a, groups, st);
-  return a.head_size == DP ? launch_mixed_form<DT, DP, WAVES, RT, false, true>(a, groups, st)
-                           : launch_mixed_form<DT, DP, WAVES, RT, true, true>(a, groups, st);
-}
-template <int DT, int DP, int WAVES>
-static int launch_mixed_waves(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
-  return a.few.rows_log2 == 4 ? launch_mixed_rows<DT, DP, WAVES, 1>(a, page16, groups, st)
-                              : launch_mixed_rows<DT, DP, WAVES, 4>(a, page16, groups, st);
+  if (!page16) return launch_mixed_form<DT, DP, RT, true, false>(a, groups, st);
+  return a.head_size == DP ? launch_mixed_form<DT, DP, RT, false, true>(a, groups, st)
+                           : launch_mixed_form<DT, DP, RT, true, true>(a, groups, st);
 }
 template <int DT, int DP>
-static int launch_mixed(const PagedAttnArgs& a, int waves, bool page16, int64_t groups, hipStream_t st) {
-  return waves == 8 ? launch_mixed_waves<DT, DP, 8>(a, page16, groups, st)
-                    : launch_mixed_waves<DT, DP, 4>(a, page16, groups, st);
+static int launch_mixed(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
+  return a.few.rows_log2 == 5 ? launch_mixed_rows<DT, DP, 2>(a, page16, groups, st)
+                              : launch_mixed_rows<DT, DP, 1>(a, page16, groups, st);
 }
 
 }  // namespace sarathi_hip

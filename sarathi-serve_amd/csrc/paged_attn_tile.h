@@ -1,25 +1,27 @@
-// Attention of a chunk of new tokens, in tiles of WAVES * 32 rows: paged_attn.h has the formulas and
-// the order of rows.
+// Attention of a chunk of new tokens, in tiles of 128 rows: paged_attn.h has the formulas and the
+// order of rows.
 //
 // Bound by the matrix cores (at the clock that their power leaves) and just below by the vector
-// unit's exponentials, so the two have to run side by side.  Each wave owns 32 rows and walks the keys
-// in steps of 64 that the workgroup shares in LDS; eight waves put two on every SIMD, so that one's
-// softmax runs beside the other's products.
+// unit's exponentials, so the two have to run side by side.  Four waves, one per SIMD, own 32 rows each
+// and walk the keys in steps of 64 that they share in LDS; two workgroups of a compute unit are not
+// tied to each other, so that one's softmax runs beside the other's products.
 //   scores  S^T = K Q^T (keys as rows, rows as columns: a row's softmax stays in two lanes), output
 //           O^T += V^T P^T; the probabilities leave the first product in the layout in which the
 //           second takes them, V is transposed by the LDS read.
 //   overlap 32 keys' softmax is cut into pieces, each placed behind the products of one operand of
 //           the NEXT 32 keys' scores; their row maximum is folded in behind the products with the
 //           values.  sched_barrier keeps the pieces apart.
-//   loads   keys and values go from global memory straight into LDS, four steps of each, two of them
-//           in flight; one barrier per step.
+//   loads   keys and values go from global memory straight into LDS, two steps of each (66 KiB: two
+//           workgroups per compute unit), asked for as soon as their place is read.
 // Chunks of 16 bytes are stored swizzled so that operand reads meet no bank twice: K by XOR with the
 // row, V by XOR of its 64-byte pieces with the row.  Built with the products' results in vector
 // registers (build.py): as accumulators they cost a move per score.
-// Measured with one chunk of 4096 tokens at 12288, 32 + 8 heads of 128, bfloat16: 955 us, 1.0 PFLOP/s,
-// where a library product of 8192^3 reaches 1.17.  Four waves of 64 rows (half the LDS reads, one
-// wave per SIMD) took 1075 us; the softmax spread evenly over both products, or a raised wave
-// priority for the second, changed nothing.
+// Measured with one chunk of 4096 tokens at 12288, 32 + 8 heads of 128, bfloat16: 0.89 - 0.92 ms,
+// 1.05 PFLOP/s, where a library product of 8192^3 reaches 1.2; with zeros for data, which leave the
+// clock alone, it runs a quarter faster.  Eight waves sharing their keys (one workgroup per compute
+// unit) were 2 % faster there, 3 % slower on four ragged chunks, 4 % on a hybrid batch and 25 % on 512
+// tokens at 8192; four waves of 64 rows (half the LDS reads, one wave per SIMD) took 1.08 ms; the
+// softmax spread evenly over both products, or a raised wave priority for the second, changed nothing.
 #pragma once
 
 #include <type_traits>
@@ -38,27 +40,26 @@ template <int DT> SK_DEV f32x16 mfma32x16(u32x4 a, u32x4 b, f32x16 c) {
 }
 
 template <int DP> struct TileShape : HeadShape<DP> {
-  static constexpr int kSteps = 4;  // of keys, and of values, in LDS at a time
+  static constexpr int kRows = 32 * kAttnWaves;
+  static constexpr int kSteps = 2;  // of keys, and of values, in LDS at a time
   static constexpr int kStepBytes = 64 * HeadShape<DP>::kRowBytes;
   static constexpr int kIdSlots = 8;
   static constexpr int kRingBytes = 2 * kSteps * kStepBytes;
-  static constexpr int kBytes = kRingBytes + 8 * kIdSlots * 64;
+  static constexpr int kBytes = kRingBytes + kAttnWaves * kIdSlots * 64;
   SK_DEV static int swz_k(int row) { return DP == 64 ? (row >> 1) & 7 : row & 15; }
   SK_DEV static int swz_v(int row) { return DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
 };
 
 SK_DEV void fence_order() { __builtin_amdgcn_sched_barrier(0); }
 
-template <int DT, int DP, int WAVES, bool PAD, bool PAGE16>
+template <int DT, int DP, bool PAD, bool PAGE16>
 SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, lds_char* lds) {
   using Sh = TileShape<DP>;
-  constexpr int ROWS = WAVES * 32, KSTEPS = DP / 16, DTILES = DP / 32;
-  constexpr int ROLES = WAVES == 8 ? 1 : 2;  // 8 waves: half of them bring keys, half values
-  constexpr int kOps = ROLES * Sh::kDmas + (PAGE16 ? 0 : 1);  // loads a wave issues per step
+  constexpr int ROWS = Sh::kRows, KSTEPS = DP / 16, DTILES = DP / 32;
+  constexpr int kOps = Sh::kDmas + (PAGE16 ? 0 : 1);  // loads a wave issues at a time
   constexpr int AHEAD = 3;                   // operands read from LDS before their products
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int share = wave & 3;
   const AttnSeq x = it.seq;
   const int32_t rows_all = x.n * a.group;
   const int32_t row0 = it.tile * ROWS;
@@ -102,34 +103,30 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
 
   const uint32_t klds = lds_addr(lds), vlds = klds + Sh::kSteps * Sh::kStepBytes;
   if constexpr (PAD) {  // chunks beyond the head are never loaded: they stay zero
-    for (int i = tid * 16; i < Sh::kRingBytes; i += WAVES * 1024)
+    for (int i = tid * 16; i < Sh::kRingBytes; i += kAttnWaves * 1024)
       *(__attribute__((address_space(3))) u32x4*)(lds + i) = u32x4{0, 0, 0, 0};
     __syncthreads();
   }
 
-  // ---- loads: a wave brings one share of the keys and one of the values of a step, or (8 waves)
-  // waves 0-3 bring keys and waves 4-7 values
+  // ---- loads: each of the four waves brings one share of the keys and one of the values of a step
   ShareLoader<DP, PAD, PAGE16, Sh::kIdSlots, false> loader{
       a, x, first, end, lane, klds + Sh::kRingBytes + (uint32_t)wave * (Sh::kIdSlots * 64)};
-  const char* src[ROLES];
-  uint32_t dst[ROLES], off[ROLES][Sh::kDmas];
+  const char* const src[2] = {reinterpret_cast<const char*>(a.k_cache) + (int64_t)h * a.head_size * 2,
+                              reinterpret_cast<const char*>(a.v_cache) + (int64_t)h * a.head_size * 2};
+  const uint32_t dst[2] = {klds + (uint32_t)wave * Sh::kShareBytes, vlds + (uint32_t)wave * Sh::kShareBytes};
+  uint32_t off[2][1][Sh::kDmas];
 #pragma unroll
-  for (int r = 0; r < ROLES; ++r) {
-    const bool keys = ROLES == 2 ? r == 0 : wave < 4;
-    src[r] = reinterpret_cast<const char*>(keys ? a.k_cache : a.v_cache) + (int64_t)h * a.head_size * 2;
-    dst[r] = (keys ? klds : vlds) + (uint32_t)share * Sh::kShareBytes;
-#pragma unroll
-    for (int n = 0; n < Sh::kDmas; ++n)
-      off[r][n] = loader.chunk(n, [&](int at) { return keys ? Sh::swz_k(at) : Sh::swz_v(at); });
+  for (int n = 0; n < Sh::kDmas; ++n) {
+    off[0][0][n] = loader.chunk(n, [](int row) { return Sh::swz_k(row); });
+    off[1][0][n] = loader.chunk(n, [](int row) { return Sh::swz_v(row); });
   }
-  auto share_at = [&](int32_t j) { return begin + j * 64 + share * 16; };
+  auto share_at = [&](int32_t j) { return begin + j * 64 + wave * 16; };
   auto load_ids = [&](int32_t j) { loader.load_ids(share_at(j), j); };
   auto share_page = [&](int32_t j) { return loader.page(share_at(j)); };
-  auto load_step = [&](int32_t j, int32_t page) {
-    uint32_t to[ROLES];
-#pragma unroll
-    for (int r = 0; r < ROLES; ++r) to[r] = dst[r] + (uint32_t)j % Sh::kSteps * Sh::kStepBytes;
-    loader.load(share_at(j), j, page, src, off, to);
+  auto load = [&](int r, int32_t j, int32_t page) {  // r: 0 keys, 1 values
+    const char* const from[1] = {src[r]};
+    const uint32_t to[1] = {dst[r] + (uint32_t)j % Sh::kSteps * Sh::kStepBytes};
+    loader.load(share_at(j), j, page, from, off[r], to);
   };
 
   // ---- operand reads
@@ -234,14 +231,19 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
   if (steps > 0) {
     if constexpr (!PAGE16) {
 #pragma unroll
-      for (int i = 0; i < 6; ++i) load_ids(i);
+      for (int i = 0; i < 4; ++i) load_ids(i);
       wait_vmcnt<0>();
     }
-    int32_t page = share_page(3);  // of the step that is asked for next
-    load_step(0, share_page(0));
-    load_step(1, share_page(1));
-    load_step(2, share_page(2));
-    wait_vmcnt<2 * ROLES * Sh::kDmas>();  // step 0
+    // pages of the steps whose values, resp. keys, are asked for next
+    int32_t page_v = share_page(1), page_k = share_page(2);
+    {
+      const int32_t page = share_page(0);
+      load(0, 0, page);
+      load(1, 0, page);
+    }
+    load(0, 1, page_v);
+    load_ids(4);
+    wait_vmcnt<Sh::kDmas + kOps>();  // keys 0
     wave_barrier();
     f32x16 s0, s1;
     {
@@ -255,23 +257,30 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s0[i]);
       raise(top);
     }
-    // Step j needs keys up to j + 1 and values j: all but what step j - 1 has asked for (before the
-    // first: step 2).
+    const std::integral_constant<int, 0> sub0{};
+    const std::integral_constant<int, 1> sub1{};
+    // Values j + 1 are asked for when values j - 1 are used up, at the start of step j, and keys j + 2
+    // when keys j are, in its middle.  Both have a step's time to land, and what is waited for is all
+    // but the last thing asked for.
     int32_t j = 0;
-    wait_vmcnt<ROLES * Sh::kDmas>();
+    wait_vmcnt<kOps>();
     while (j + 1 < steps) {
       wave_barrier();
-      load_step(j + 3, page);
-      load_ids(j + 6);
-      page = share_page(j + 4);
-      body(2 * j, std::integral_constant<int, 0>{}, s0, s1, std::true_type{});
-      body(2 * j + 1, std::integral_constant<int, 1>{}, s1, s0, std::true_type{});
+      load(1, j + 1, page_v);
+      body(2 * j, sub0, s0, s1, std::true_type{});
+      wait_vmcnt<Sh::kDmas>();
+      wave_barrier();
+      load(0, j + 2, page_k);
+      load_ids(j + 5);
+      page_v = page_k;
+      page_k = share_page(j + 3);
+      body(2 * j + 1, sub1, s1, s0, std::true_type{});
       wait_vmcnt<kOps>();
       ++j;
     }
     wave_barrier();
-    body(2 * j, std::integral_constant<int, 0>{}, s0, s1, std::true_type{});
-    body(2 * j + 1, std::integral_constant<int, 1>{}, s1, s0, std::false_type{});
+    body(2 * j, sub0, s0, s1, std::true_type{});
+    body(2 * j + 1, sub1, s1, s0, std::false_type{});
     wait_vmcnt<0>();  // nothing may land in LDS after this workgroup has left it
   }
 
