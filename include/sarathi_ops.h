@@ -405,9 +405,10 @@ int sarathi_build_paged_kv_metadata(const int32_t* query_lens, const int32_t* se
  *
  * Lengths are read on the GPU, so a captured call follows what the index vectors hold at replay.
  * Index vectors must not decrease; whatever they hold, nothing outside the tensors is touched, and
- * a page number outside [0, num_pages) is not followed (the last page stands in for it).  Entries
- * past a request's last key are not read; entries of the request itself that a mask hides from some
- * of its tokens must be finite.
+ * a page number outside [0, num_pages) is not followed (the last page stands in for it).  Keys and
+ * values past a request's last one, or in front of what a window shows to any of its tokens, are not
+ * read.  A value that some of a request's tokens see and a mask hides from others must be finite:
+ * otherwise the others may become NaN too.  out and lse must not overlap the other tensors.
  *
  * max_query_len (0: unknown) is an upper bound of the new tokens of any request; it picks the
  * kernel, and a wrong one costs time, not correctness.  workspace: scratch of

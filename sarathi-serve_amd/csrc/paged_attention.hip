@@ -345,6 +345,8 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   p.few.target = (int32_t)few_target;
   p.tile.target = (int32_t)chunk_target;
   p.few.row_base = (int32_t)chunk_rows;
+  p.few.most = (int32_t)(few_tiles + few_target);
+  p.tile.most = (int32_t)(chunk_tiles + chunk_target);
   p.map_bytes = round256((2 * seqs + 1) * 4);
   p.ml_bytes = round256(state_rows * 8);
   p.o_bytes = round256(state_rows * head_size * 4);

@@ -35,6 +35,7 @@ struct AttnClass {
   int32_t fill;       // items per key head that fill the GPU once
   int32_t min_part;   // least keys of a part, a multiple of 64
   int32_t row_base;   // first state row of the class
+  int32_t most;       // items there is room for in the states; sound index vectors stay within
 };
 
 struct PagedAttnArgs {
@@ -259,10 +260,16 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   const uint32_t in_class = tiled ? tiles_before : want - tiles_before;
   int32_t cut = 0;
   each([&](int32_t r, const Load& v) {
-    const int32_t parts = parts_of(v);
-    const uint32_t cnt = (uint32_t)(v.tiles * parts);
+    int32_t parts = parts_of(v);
+    uint32_t cnt = (uint32_t)(v.tiles * parts);
     uint32_t& mine_at = v.tiled ? tile_at : few_at;
     const AttnClass& c = v.tiled ? a.tile : a.few;
+    // index vectors that decrease can ask for more states than there are: such a request is left out
+    if (parts > 1 && mine_at + (uint64_t)v.tiles * (uint32_t)parts > (uint32_t)c.most) {
+      mine_at += cnt;
+      cnt = 0;
+      parts = 1;
+    }
     const int32_t state = c.row_base + (int32_t)((mine_at * (uint32_t)a.kv_heads) << c.rows_log2);
     if (map) {
       a.part_map[r] = state;

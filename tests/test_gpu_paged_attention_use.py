@@ -256,7 +256,7 @@ def test_refusals(ops, dev):
 
 # ---- the C ABI ----------------------------------------------------------------------------------
 
-def _abi_attention(lib, d, out, ws, ws_bytes, scale):
+def _abi_attention(lib, d, out, ws, ws_bytes, scale, hint=0):
     q, c = d["query"], d["cache"]
     return lib.sarathi_paged_attention(
         abi.ptr(q), abi.ptr(c), abi.vp(c.data_ptr() + c.stride(1) * 2), abi.ptr(out), abi.vp(None),
@@ -264,7 +264,7 @@ def _abi_attention(lib, d, out, ws, ws_bytes, scale):
         abi.i64(q.shape[0]), abi.i64(d["last"].numel()), abi.i64(d["kv_indices"].numel()), abi.i64(c.shape[0]),
         abi.ci(q.shape[1]), abi.ci(c.shape[3]), abi.ci(c.shape[4]), abi.ci(c.shape[2]), abi.i64(q.stride(0)),
         abi.i64(out.stride(0)), abi.i64(c.stride(0)), abi.i64(c.stride(2)), abi.cf(scale), abi.ci(1), abi.i64(-1),
-        abi.i64(0), ws, abi.i64(ws_bytes), abi.ci(abi.DT[q.dtype]), abi.stream())
+        abi.i64(hint), ws, abi.i64(ws_bytes), abi.ci(abi.DT[q.dtype]), abi.stream())
 
 
 def test_without_a_workspace_nothing_is_cut(ops, dev):
@@ -598,3 +598,46 @@ def test_merge_strides(ops, dev, states):
     odd[:, :, 3:] = v.transpose(0, 1).flatten(2)
     e, _ = ops.kv_cache_ops.merge_attention_states(odd[:, :, 3:].unflatten(2, (6, 64)), z.transpose(0, 1))
     assert bool(((e.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-6).all())
+
+
+# ---- what reviews of the kernels asked for --------------------------------------------------------
+
+@pytest.mark.parametrize("hint", [0, 8])
+def test_decreasing_index_vectors_stay_inside_the_workspace(ops, dev, hint):
+    """Index vectors that decrease name more tiles than the tensors' sizes allow for: the states that
+    cutting leaves in the workspace stay within it (the memory on both sides is left as it was)."""
+    lib = abi.load()
+    T, N, D, S = 64, 300, 64, 33
+    d = dict(query=torch.ones((T, 8, D), dtype=torch.bfloat16, device=dev),
+             cache=torch.ones((N, 2, 16, 1, D), dtype=torch.bfloat16, device=dev),
+             qo_indptr=torch.tensor([0, T] * ((S + 1) // 2), dtype=torch.int32, device=dev),
+             kv_indptr=torch.tensor([0, N] * ((S + 1) // 2), dtype=torch.int32, device=dev),
+             kv_indices=torch.arange(N, dtype=torch.int32, device=dev),
+             last=torch.full((S,), 16, dtype=torch.int32, device=dev))
+    need = lib.sarathi_paged_attention_workspace_bytes
+    need.restype = ctypes.c_int64
+    bytes_ = need(abi.i64(T), abi.i64(S), abi.i64(N), abi.ci(8), abi.ci(1), abi.ci(D), abi.ci(16), abi.i64(hint))
+    assert bytes_ > 0
+    guard = 1 << 24
+    ws = torch.full((bytes_ + 2 * guard,), 77, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(d["query"])
+    abi.check(lib, _abi_attention(lib, d, out, abi.vp(ws.data_ptr() + guard), bytes_, D ** -0.5, hint))
+    torch.cuda.synchronize()
+    assert bool((ws[:guard] == 77).all()) and bool((ws[guard + bytes_:] == 77).all())
+
+
+@pytest.mark.parametrize("new,heads,D,page", [(1, 8, 128, 16), (60, 8, 128, 16), (1, 4, 64, 5), (70, 4, 64, 24)])
+def test_pages_behind_the_window_may_be_gone(ops, dev, new, heads, D, page):
+    """Keys that the window hides from every token are not read: their pages may hold anything, or no
+    longer be named."""
+    total, window = 1333, 300
+    b = build_batch(41, page, [new], [total], heads, 1, D, torch.bfloat16)
+    want = reference(b, window=window)
+    first = total - new - window                                  # first key that any token sees
+    flat = b["cache"][b["kv_indices"].long()].clone()             # pages in order
+    for t in range(first):
+        flat[t // page, :, t % page] = float("nan")
+    b["cache"][b["kv_indices"].long()] = flat
+    b["kv_indices"][:first // page] = -1
+    got, lse = call(ops, dev, b, window_left=window, return_lse=True)
+    check(b, got, lse, want)
