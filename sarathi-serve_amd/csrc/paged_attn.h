@@ -500,10 +500,12 @@ template <int DP, bool PAD, bool PAGE16, int IDS, bool ONCE> struct ShareLoader 
 };
 
 // The running maximum of a row is only a reference for its exponents, and it is raised only when a
-// score passes it by more than 2^kRaise: probabilities then stay below 2^8, which neither 16-bit type
-// nor the 32-bit sums mind, and the output is almost never rescaled.
+// score passes the one it was set for by more than 2^8, so the output is almost never rescaled.  It is
+// set kBelow under that score: probabilities stay below 2^8 in bfloat16 and, to use the range of
+// float16 (which ends at 2^-24), below 2^15 there; the 32-bit sums mind neither.
 constexpr float kRefStart = -3.0e38f;  // below every score; finite, so that no difference is undefined
-constexpr float kRaise = 8.f;
+template <int DT> constexpr float kBelow = DT == kF16 ? 7.f : 0.f;
+template <int DT> constexpr float kRaise = 8.f + kBelow<DT>;
 
 // lse of a state with reference m (in powers of two) and sum l; -inf where nothing was seen
 SK_DEV float attn_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }

@@ -170,12 +170,12 @@ SK_DEV void few_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, lds
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       z[rt] = group_max(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]))) * a.scale_log2;
-      need |= z[rt] > ref[rt] + kRaise;
+      need |= z[rt] > ref[rt] + kRaise<DT>;
     }
     if (__builtin_amdgcn_ballot_w64(need) != 0) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float next = fmaxf(ref[rt], z[rt]);
+        const float next = fmaxf(ref[rt], z[rt] - kBelow<DT>);
         const float keep = __builtin_amdgcn_exp2f(ref[rt] - next);
         ref[rt] = next;
         l[rt] *= keep;

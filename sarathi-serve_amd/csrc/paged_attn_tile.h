@@ -166,8 +166,8 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
   auto raise = [&](float top) {
     auto w = __builtin_amdgcn_permlane32_swap(as_u32(top), as_u32(top), false, false);
     const float z = fmaxf(as_f32(w[0]), as_f32(w[1])) * a.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(z > ref + kRaise) == 0) return;
-    const float next = fmaxf(ref, z);
+    if (__builtin_amdgcn_ballot_w64(z > ref + kRaise<DT>) == 0) return;
+    const float next = fmaxf(ref, z - kBelow<DT>);
     const float keep = __builtin_amdgcn_exp2f(ref - next);
     ref = next;
     l *= keep;

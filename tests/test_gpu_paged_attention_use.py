@@ -626,6 +626,30 @@ def test_decreasing_index_vectors_stay_inside_the_workspace(ops, dev, hint):
     assert bool((ws[:guard] == 77).all()) and bool((ws[guard + bytes_:] == 77).all())
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_small_probabilities_keep_their_share_in_float16(ops, dev, new):
+    """One key far above all others: theirs are 2^-25.5 of it, below half of float16's least step, and
+    only they have values.  They are held 2^7 higher, where a step is 2^-24 / 2^-18.5 = 2.2 % of one:
+    half of it, and half a step of the result (2^-25), is the bound."""
+    keys, D = 1500, 64
+    d = dict(query=torch.zeros((new, 4, D), dtype=torch.float16, device=dev),
+             cache=torch.zeros((94, 2, 16, 1, D), dtype=torch.float16, device=dev),
+             qo_indptr=torch.tensor([0, new], dtype=torch.int32, device=dev),
+             kv_indptr=torch.tensor([0, 94], dtype=torch.int32, device=dev),
+             kv_indices=torch.arange(94, dtype=torch.int32, device=dev),
+             last=torch.tensor([keys - 93 * 16], dtype=torch.int32, device=dev))
+    d["query"][..., 0] = 25.5
+    d["cache"][:, 1] = 1024.0
+    d["cache"][:4, 0, :, :, 0] = 1.0       # the 64 first keys, one block of every wave
+    d["cache"][:4, 1] = 0.0
+    out = ops.kv_cache_ops.paged_attention(d["query"], d["cache"], d["qo_indptr"], d["kv_indptr"], d["kv_indices"],
+                                           d["last"], sm_scale=float(np.log(2.0)), causal=False)
+    small = (keys - 64) * 2.0 ** -25.5
+    want = 1024 * small / (64 + small)
+    got = out.cpu().double()
+    assert bool(((got - want).abs() <= 2.0 ** -6.5 * want + 2.0 ** -25).all()), (got.min().item(), want)
+
+
 @pytest.mark.parametrize("new,heads,D,page", [(1, 8, 128, 16), (60, 8, 128, 16), (1, 4, 64, 5), (70, 4, 64, 24)])
 def test_pages_behind_the_window_may_be_gone(ops, dev, new, heads, D, page):
     """Keys that the window hides from every token are not read: their pages may hold anything, or no
