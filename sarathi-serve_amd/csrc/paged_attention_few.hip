@@ -28,9 +28,11 @@ static int launch_few(const PagedAttnArgs& a, int64_t groups, hipStream_t st) {
 // the exact head size and pages of a multiple of 16 keys have kernels of their own
 template <int DT, int DP, int RT>
 static int launch_few_form(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
-  if (!page16) return launch_few<DT, DP, RT, true, false>(a, groups, st);
-  return a.head_size == DP ? launch_few<DT, DP, RT, false, true>(a, groups, st)
-                           : launch_few<DT, DP, RT, true, true>(a, groups, st);
+  if (a.head_size < DP)
+    return page16 ? launch_few<DT, DP, RT, true, true>(a, groups, st)
+                  : launch_few<DT, DP, RT, true, false>(a, groups, st);
+  return page16 ? launch_few<DT, DP, RT, false, true>(a, groups, st)
+                : launch_few<DT, DP, RT, false, false>(a, groups, st);
 }
 template <int DT, int DP>
 static int launch_few_rows(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {

@@ -34,9 +34,11 @@ static int launch_mixed_form(const PagedAttnArgs& a, int64_t groups, hipStream_t
 }
 template <int DT, int DP, int RT>
 static int launch_mixed_rows(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
-  if (!page16) return launch_mixed_form<DT, DP, RT, true, false>(a, groups, st);
-  return a.head_size == DP ? launch_mixed_form<DT, DP, RT, false, true>(a, groups, st)
-                           : launch_mixed_form<DT, DP, RT, true, true>(a, groups, st);
+  if (a.head_size < DP)
+    return page16 ? launch_mixed_form<DT, DP, RT, true, true>(a, groups, st)
+                  : launch_mixed_form<DT, DP, RT, true, false>(a, groups, st);
+  return page16 ? launch_mixed_form<DT, DP, RT, false, true>(a, groups, st)
+                : launch_mixed_form<DT, DP, RT, false, false>(a, groups, st);
 }
 template <int DT, int DP>
 static int launch_mixed(const PagedAttnArgs& a, bool page16, int64_t groups, hipStream_t st) {
