@@ -16,7 +16,9 @@
 // is ONE launch of independent workgroups, each of one request (or of a piece of a long one): it adds
 // up the lengths of the requests before its own (all of them come out of L2), and then its tokens and
 // pages lie side by side, so nothing is searched for.  The additions grow with the square of the
-// requests; beyond the limit one workgroup writes the prefix sums first.
+// requests; beyond the limit one workgroup writes the prefix sums first.  Measured: 16 decodes 4.4 us,
+// 1008 requests with 2304 tokens and tables of 512 pages 6.8 us, of which an empty launch takes 1.6;
+// the call costs 8 us of host time (eight tensors out of one allocation).
 #include "launch.h"
 #include "vec16.h"
 

@@ -88,7 +88,8 @@ __global__ __launch_bounds__(64) void paged_attn_plain_kernel(PagedAttnArgs a) {
 // rows and their parts: with few rows several take turns at one row's parts, and each has eight of them on
 // their way at once, so that the time hardly grows with the parts.  A part whose sum is zero has no
 // output.  Parts are added in a fixed order: results do not depend on which workgroup ran when.
-// Nothing to join (the attention kernel leaves word) costs a launch and one load.
+// Nothing to join (the attention kernel leaves word) costs a launch and one load.  Bound by latency: 4 to
+// 7 us from one request to 256, of which up to 4 hide behind the kernel before.
 constexpr int kJoinRows = 4;
 
 template <int DT, int VALS, int WPT>  // VALS elements of the head per lane

@@ -1,5 +1,4 @@
-// Pieces shared by the kernels that attend over a paged KV cache (paged_attention.hip,
-// paged_attention_tiles.hip).
+// Pieces shared by the kernels that attend over a paged KV cache (paged_attention*.hip).
 //
 // For a request with n new tokens whose sequence holds s tokens after the append, new token j sits
 // at position x = s - n + j and sees the keys [lo, hi):
@@ -248,8 +247,8 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     tile_items += sums[1][w];
   }
   // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
-  // are at work all the time; the last quarter of the few ones evens out the end.  Batch of 2304
-  // tokens: 876 us, 945 with all tiles first.
+  // are at work all the time; the last quarter of the few ones evens out the end.  A chunk of 2048
+  // tokens beside 256 decodes: 7 % faster than with all tiles first.
   const uint32_t mixed = tile_items + (uint32_t)((uint64_t)few_items * 3 / 4);
   uint32_t tiles_before = tile_items;
   bool tiled = false;
