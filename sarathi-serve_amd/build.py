@@ -26,8 +26,10 @@ HIP_SOURCES = ["rms_norm.hip", "gated_act.hip", "rope.hip", "moe_topk.hip", "moe
                "moe_fused_routing.hip", "stream_copy.hip", "moe_balance.hip", "moe_gemm_f32.hip",
                "moe_gemm_rider.hip", "kv_metadata.hip", "paged_attention.hip",
                "paged_attention_few.hip", "paged_attention_mixed_bf16_64.hip",
-               "paged_attention_mixed_bf16_128.hip", "paged_attention_mixed_f16_64.hip",
-               "paged_attention_mixed_f16_128.hip", "merge_states.hip"]
+               "paged_attention_mixed_bf16_128.hip", "paged_attention_mixed_bf16_256.hip",
+               "paged_attention_mixed_f16_64.hip",
+               "paged_attention_mixed_f16_128.hip", "paged_attention_mixed_f16_256.hip",
+               "merge_states.hip"]
 CXX_SOURCES = ["abi_misc.cpp"]
 
 ABI_LIB = os.path.join(LIB_DIR, "libsarathi_ops_hip.so")

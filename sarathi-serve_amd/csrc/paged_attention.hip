@@ -293,10 +293,12 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   const int64_t units = compute_units();
   const int few_limit = head_size > 128 ? 32 : 64;
   int64_t few_tiles = 0, chunk_tiles = 0, few_target = 0, chunk_target = 0;
-  // two workgroups per compute unit
-  p.few.fill = p.tile.fill = 2 * units / kv_heads > 0 ? (int32_t)(2 * units / kv_heads) : 1;
+  // two workgroups per compute unit; one where a chunk's tile has long heads
+  const int64_t room = 2 * units, tile_room = head_size > 128 ? units : room;
+  p.few.fill = room / kv_heads > 0 ? (int32_t)(room / kv_heads) : 1;
+  p.tile.fill = tile_room / kv_heads > 0 ? (int32_t)(tile_room / kv_heads) : 1;
   p.few.rows_log2 = p.tile.rows_log2 = -1;
-  if (most_rows <= few_limit || head_size > 128) {
+  if (most_rows <= few_limit) {
     // all requests in tiles of few rows (max_query_len may be wrong: any number of tiles each)
     const int rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : few_limit;
     p.few.rows_log2 = log2_of(rows);
@@ -316,7 +318,7 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
     chunk_tiles = all_rows / big + chunks;
     // cut only where the tiles leave a quarter of the GPU idle: a part costs its state's way to
     // memory and back
-    if (all_rows / big * kv_heads < 2 * units * 3 / 4) chunk_target = p.tile.fill;
+    if (all_rows / big * kv_heads < tile_room * 3 / 4) chunk_target = p.tile.fill;
     p.tile.min_part = 512;
   }
   if (few_tiles > all_rows) few_tiles = all_rows;
@@ -358,17 +360,18 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
 
 using namespace sarathi_hip;
 
-// Heads of up to 128 in batches that may hold chunks take the kernel that does both classes; the
-// others have few rows only.
+// Batches that may hold chunks take the kernel that does both classes; the others have few rows only.
 static int launch_paged_attn(const PagedAttnArgs& a, int dtype, bool page16, int64_t groups,
                              hipStream_t st) {
   if (groups == 0) return SARATHI_OK;
   if (a.tile.rows_log2 < 0) return launch_attn_few(a, dtype, page16, groups, st);
   if (dtype == kBF16)
-    return a.head_size <= 64 ? launch_attn_mixed_bf16_64(a, page16, groups, st)
-                             : launch_attn_mixed_bf16_128(a, page16, groups, st);
-  return a.head_size <= 64 ? launch_attn_mixed_f16_64(a, page16, groups, st)
-                           : launch_attn_mixed_f16_128(a, page16, groups, st);
+    return a.head_size <= 64    ? launch_attn_mixed_bf16_64(a, page16, groups, st)
+           : a.head_size <= 128 ? launch_attn_mixed_bf16_128(a, page16, groups, st)
+                                : launch_attn_mixed_bf16_256(a, page16, groups, st);
+  return a.head_size <= 64    ? launch_attn_mixed_f16_64(a, page16, groups, st)
+         : a.head_size <= 128 ? launch_attn_mixed_f16_128(a, page16, groups, st)
+                              : launch_attn_mixed_f16_256(a, page16, groups, st);
 }
 
 static bool attn_sizes_ok(int64_t tokens, int64_t seqs, int64_t indices, int heads, int kv_heads,

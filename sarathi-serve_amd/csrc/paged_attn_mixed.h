@@ -1,7 +1,7 @@
 // The attention kernel of hybrid batches: one launch whose work items are the tiles of the chunks and
 // those of the decode tokens, in turn.  Chunks are bound by the matrix cores and decodes by memory, so
 // some compute units stream keys and values while the others multiply.  Both kinds of item take half
-// a compute unit: four waves, one per SIMD, and 66 KiB of LDS.
+// a compute unit: four waves, one per SIMD, and 66 KiB of LDS (heads above 128: a whole one, 130 KiB).
 #pragma once
 
 #include "launch.h"
@@ -12,7 +12,7 @@
 namespace sarathi_hip {
 
 template <int DT, int DP, int RT, bool PAD, bool PAGE16>
-__global__ __launch_bounds__(64 * kAttnWaves) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(64 * kAttnWaves) __attribute__((amdgpu_waves_per_eu(DP <= 128 ? 2 : 1, DP <= 128 ? 2 : 1)))
 void paged_attn_mixed_kernel(PagedAttnArgs a) {
   extern __shared__ u32x4 mixed_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;

@@ -12,7 +12,8 @@
 //           the NEXT 32 keys' scores; their row maximum is folded in behind the products with the
 //           values.  sched_barrier keeps the pieces apart.
 //   loads   keys and values go from global memory straight into LDS, two steps of each (66 KiB: two
-//           workgroups per compute unit), asked for as soon as their place is read.
+//           workgroups per compute unit; 130 KiB and one with heads above 128), asked for as soon as
+//           their place is read.  Four steps of each made short chunks no faster.
 // Chunks of 16 bytes are stored swizzled so that operand reads meet no bank twice: K by XOR with the
 // row, V by XOR of its 64-byte pieces with the row.  Built with the products' results in vector
 // registers (build.py): as accumulators they cost a move per score.
@@ -22,6 +23,8 @@
 // unit) were 2 % faster there, 3 % slower on four ragged chunks, 4 % on a hybrid batch and 25 % on 512
 // tokens at 8192; four waves of 64 rows (half the LDS reads, one wave per SIMD) took 1.08 ms; the
 // softmax spread evenly over both products, or a raised wave priority for the second, changed nothing.
+// Heads of 256, 64 + 8 of them, 4096 tokens at 4096: 1.64 ms, 1.01 PFLOP/s (4.72 ms in tiles of 32 rows).
+// A launch of few tiles is bound by the chain of a wave alone on its SIMD: 1.4 us per 64 keys and tile.
 #pragma once
 
 #include <type_traits>
@@ -180,8 +183,9 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
     constexpr bool MORE = decltype(more)::value;
     constexpr int SUB = decltype(sub)::value;
     constexpr int PV = 2 * DTILES;       // operands of the output's products
-    constexpr int PER = 16 / KSTEPS;     // probabilities per operand of the next scores
-    constexpr int PERM = 16 / PV;        // scores that enter the maximum per operand
+    // pairs of probabilities are made behind the operands of the next scores, and pairs of scores
+    // enter the maximum behind those of the output: as many of the eight by the n-th of `all`
+    auto pairs_by = [](int n, int all) { return n * 8 / all; };
     const uint32_t v_at = (uint32_t)u / 2 % Sh::kSteps * Sh::kStepBytes;
     const uint32_t k_at = ((uint32_t)u + 1) / 2 % Sh::kSteps * Sh::kStepBytes;
     u32x4 p[2], kf[AHEAD + 1], vf[AHEAD + 1];
@@ -202,7 +206,7 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
         vf[i] = read_v(v_at, SUB, i / DTILES, i % DTILES);
       }
 #pragma unroll
-      for (int i = n * PER; i < (n + 1) * PER; i += 2) {
+      for (int i = 2 * pairs_by(n, KSTEPS); i < 2 * pairs_by(n + 1, KSTEPS); i += 2) {
         const float z0 = __builtin_amdgcn_exp2f(fmaf(cur[i], a.scale_log2, -ref));
         const float z1 = __builtin_amdgcn_exp2f(fmaf(cur[i + 1], a.scale_log2, -ref));
         l += z0 + z1;
@@ -221,7 +225,7 @@ SK_DEV void tile_item(const PagedAttnArgs& a, const AttnItem& it, uint32_t h, ld
       o[n % DTILES] = mfma32x16<DT>(vf[n % (AHEAD + 1)], p[n / DTILES], o[n % DTILES]);
       if constexpr (MORE) {
 #pragma unroll
-        for (int i = n * PERM; i < (n + 1) * PERM; i += 2) top = fmaxf(fmaxf(top, next[i]), next[i + 1]);
+        for (int i = 2 * pairs_by(n, PV); i < 2 * pairs_by(n + 1, PV); i += 2) top = fmaxf(fmaxf(top, next[i]), next[i + 1]);
       }
       fence_order();
     }

@@ -665,3 +665,17 @@ def test_pages_behind_the_window_may_be_gone(ops, dev, new, heads, D, page):
     b["kv_indices"][:first // page] = -1
     got, lse = call(ops, dev, b, window_left=window, return_lse=True)
     check(b, got, lse, want)
+
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,head_size,page,dtype,kw", [
+    ([300], [1700], 12, 4, 256, 16, torch.bfloat16, {}),
+    ([300, 1, 40], [300, 2000, 1999], 8, 1, 256, 7, torch.float16, {}),                 # cut, odd pages
+    ([129, 1], [900, 64], 40, 2, 192, 32, torch.bfloat16, dict(window_left=200)),
+    ([70, 2, 1], [70, 1, 90], 3, 3, 136, 16, torch.float16, dict(causal=False)),
+    ([40], [2600], 2, 1, 200, 5, torch.bfloat16, {}),
+])
+def test_chunks_of_long_heads(ops, dev, new, total, heads, kv_heads, head_size, page, dtype, kw):
+    b = build_batch(43, page, new, total, heads, kv_heads, head_size, dtype)
+    got, lse = call(ops, dev, b, return_lse=True, **kw)
+    check(b, got, lse, reference(b, kw.get("causal", True), kw.get("window_left", -1)))
+    assert torch.equal(call(ops, dev, b, **kw), got)
