@@ -39,12 +39,12 @@ def attend(ops, d, **kw):
     # a chunk whose few tiles are cut as well
     ([70], [4200], 4, 1, 128, 16, torch.bfloat16, {}),
     ([33, 1, 40], [2100, 900, 3000], 8, 1, 64, 16, torch.float16, dict(window_left=1500)),
-    # 256-row tiles: ragged, windows inside a chunk, pages that are no multiple of 16
+    # large tiles: ragged, windows inside a chunk, pages that are no multiple of 16
     ([1100, 1, 900, 1], [1100, 300, 1500, 17], 16, 16, 64, 16, torch.bfloat16, {}),
     ([700], [1700], 32, 16, 128, 16, torch.bfloat16, dict(window_left=130)),
     ([513], [600], 64, 8, 128, 24, torch.float16, {}),
     ([400, 0, 1], [450, 12, 77], 48, 8, 96, 16, torch.bfloat16, dict(causal=False)),
-    # a head size without a matrix-core tile for chunks
+    # a head size between those of the tiles
     ([150, 1], [260, 700], 6, 2, 192, 16, torch.bfloat16, {}),
     # query heads per key head above 16 and above 64
     ([1, 9, 1], [300, 200, 2], 34, 2, 128, 16, torch.bfloat16, {}),
