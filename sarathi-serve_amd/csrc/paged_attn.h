@@ -108,6 +108,8 @@ SK_DEV int64_t attn_entry(const PagedAttnArgs& a, const AttnSeq& x, int32_t pos)
 
 constexpr int kPartKeys = 1024;
 constexpr int kCutKeys = 512;
+constexpr int kBins = 4;
+constexpr int kSortRounds = 10;
 
 struct AttnItem {
   int32_t r;         // request, -1: none
@@ -139,8 +141,10 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
   return a.window >= 0 && s < x.s ? (int32_t)s : x.s;
 }
 
-// Finds item `want` of a key head: first the tiles of the chunks, then those of few rows, each in
-// the order request, tile, part.  Two sums over the requests: keys times tiles of either class,
+// Finds item `want` of a key head: tiles of the chunks, in the order request, tile, part, and in between
+// those of few rows, sorted by length into kBins bins, the longest first, so that the end is even (256
+// requests: 5 % faster), unless they are short, all there at once, or so many (kSortRounds times what fills the GPU)
+// that the short ones in a row cost more (1000 requests: 4 % slower).  Two sums over the requests: keys times tiles of either class,
 // which fix the classes' part lengths, and the numbers of items.  A part is as long as filling the
 // GPU once allows but no longer than kPartKeys (below, its start and the way of its state to memory
 // and back weigh in), unless that made more than `target` items; it is at least min_part keys and a
@@ -152,7 +156,7 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
   constexpr int WAVES = kAttnWaves;
   __shared__ float work_sums[2][2][WAVES];
-  __shared__ uint32_t sums[2][WAVES];
+  __shared__ u32x4 sums[3];  // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3
   __shared__ AttnItem found;
   constexpr int NT = WAVES * 64, KEEP = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -160,7 +164,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   const int64_t first = (int64_t)tid * run;
   const int32_t r0 = first < a.seqs ? (int32_t)first : a.seqs;
   const int32_t r1 = first + run < a.seqs ? (int32_t)(first + run) : a.seqs;
-  struct Load { int32_t tiles, keys; bool tiled; AttnSeq seq; };
+  struct Load { int32_t tiles, keys; bool tiled; AttnSeq seq; int32_t parts; };
   auto look = [&](int32_t r) {
     const AttnSeq x = attn_seq(a, r);
     const int64_t rows = (int64_t)x.n * a.group;
@@ -170,22 +174,28 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     v.tiles = (int32_t)((rows + ((int64_t)1 << lg) - 1) >> lg);
     v.keys = attn_keys(a, x);
     v.seq = x;
+    v.parts = 0;
     return v;
   };
   Load kept[KEEP];  // the first requests of this thread are looked at once
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
-    kept[i] = {0, 0, false, {0, 0, 0, 0}};
+    kept[i] = {0, 0, false, {0, 0, 0, 0}, 0};
     if (r0 + i < r1) kept[i] = look(r0 + i);
   }
   auto each = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       if (r0 + i < r1) f(r0 + i, kept[i]);
-    for (int32_t r = r0 + KEEP; r < r1; ++r) f(r, look(r));
+    for (int32_t r = r0 + KEEP; r < r1; ++r) {
+      Load v = look(r);
+      f(r, v);
+    }
   };
   if (tid == 0) found.r = -1;
   int32_t few_len = 0x7fffffff, tile_len = 0x7fffffff;
+  bool sorted = false;    // items of few rows, into bins
+  float per_block = 0.f;  // bins per 64 keys
   if (a.few.target > 0 || a.tile.target > 0) {
     float few = 0.f, tile = 0.f, few_most = 0.f, tile_most = 0.f;  // keys times tiles; longest
     each([&](int32_t, const Load& v) {
@@ -214,37 +224,85 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
         most = fmaxf(most, sum[1][w]);
       }
       work *= 1.001f;
-      const float len = fmaxf(fminf(work / (float)c.fill, kPartKeys / 64), work / (float)c.target);
+      const float len = fmaxf(fminf(work * __builtin_amdgcn_rcpf((float)c.fill), kPartKeys / 64),
+                              work * __builtin_amdgcn_rcpf((float)c.target));
       if (most <= len + kCutKeys / 64) return 0x7fffffff;
       const int32_t keys = len > 1.6e7f ? 0x3fffffc0 : (int32_t)ceilf(len) * 64;
       return keys > c.min_part ? keys : c.min_part;
     };
     few_len = length(work_sums[0], a.few);
     tile_len = length(work_sums[1], a.tile);
+    float work = 0.f, longest = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      work += work_sums[0][0][w];
+      longest = fmaxf(longest, work_sums[0][1][w]);
+    }
+    const float len = fminf(longest, (float)(few_len >> 6));
+    sorted = __builtin_amdgcn_readfirstlane(
+        a.few.target > 0 && a.few.most <= 0xffff &&  // bins count in 16 bits
+        longest > kPartKeys / 64 && work > len * (float)(a.few.fill - a.seqs) &&
+        work <= len * (float)(kSortRounds * a.few.fill - a.seqs));
+    per_block = kBins * __builtin_amdgcn_rcpf(len + 1.f);
   }
+  auto bin_of = [&](int32_t keys) {
+    const int32_t b = (int32_t)((float)((keys >> 6) + 1) * per_block);
+    return b < kBins - 1 ? b : kBins - 1;
+  };
+  // items in bin b of packed counts (those that are not sorted are one number, in the first word)
+  auto in_bin = [](uint32_t c01, uint32_t c23, int b) { return ((b < 2 ? c01 : c23) >> (16 * (b & 1))) & 0xffffu; };
   auto parts_of = [&](const Load& v) {
     const int32_t len = v.tiled ? tile_len : few_len;
     return v.keys <= len ? 1 : (v.keys - 1) / len + 1;
   };
-  uint32_t my_few = 0, my_tile = 0;
-  each([&](int32_t, const Load& v) { (v.tiled ? my_tile : my_few) += (uint32_t)(v.tiles * parts_of(v)); });
-  uint32_t few_at = wave_scan(my_few), tile_at = wave_scan(my_tile);
-  if (lane == 63) {
-    sums[0][wave] = few_at;
-    sums[1][wave] = tile_at;
-  }
-  few_at -= my_few;
-  tile_at -= my_tile;
-  __syncthreads();
-  uint32_t few_items = 0, tile_items = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) {
-      few_at += sums[0][w];
-      tile_at += sums[1][w];
+  // the whole parts of a request of few rows, and the rest of each tile
+  auto whole_bin = [&](int32_t parts) { return parts > 1 ? bin_of(few_len) : 0; };
+  auto rest_bin = [&](const Load& v, int32_t parts) {
+    return bin_of(parts > 1 ? v.keys - (parts - 1) * few_len : v.keys);
+  };
+  uint32_t my_tile = 0, my01 = 0, my23 = 0;
+  auto add = [&](int32_t b, uint32_t n) { (b < 2 ? my01 : my23) += n << (16 * (b & 1)); };
+  each([&](int32_t, Load& v) {
+    v.parts = parts_of(v);
+    if (v.tiled) {
+      my_tile += (uint32_t)(v.tiles * v.parts);
+    } else if (sorted) {
+      add(whole_bin(v.parts), (uint32_t)(v.tiles * (v.parts - 1)));
+      add(rest_bin(v, v.parts), (uint32_t)v.tiles);
+    } else {
+      my01 += (uint32_t)(v.tiles * v.parts);
     }
-    few_items += sums[0][w];
-    tile_items += sums[1][w];
+  });
+  uint32_t tile_at = wave_scan(my_tile), at01 = wave_scan(my01), at23 = 0;
+  if (sorted) at23 = wave_scan(my23);
+  if (lane == 63) {
+    ((uint32_t*)&sums[0])[wave] = tile_at;
+    ((uint32_t*)&sums[1])[wave] = at01;
+    ((uint32_t*)&sums[2])[wave] = at23;
+  }
+  tile_at -= my_tile;
+  at01 -= my01;
+  at23 -= my23;
+  __syncthreads();
+  uint32_t tile_items = 0, all01 = 0, all23 = 0;
+  {
+    const u32x4 t = sums[0], c = sums[1], d = sums[2];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) {
+        tile_at += t[w];
+        at01 += c[w];
+        at23 += d[w];
+      }
+      tile_items += t[w];
+      all01 += c[w];
+      all23 += d[w];
+    }
+  }
+  uint32_t few_items = all01, few_at = at01;
+  if (sorted) {
+    few_items = (all01 & 0xffffu) + (all01 >> 16) + (all23 & 0xffffu) + (all23 >> 16);
+    few_at = (at01 & 0xffffu) + (at01 >> 16) + (at23 & 0xffffu) + (at23 >> 16);
   }
   // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
   // are at work all the time; the last quarter of the few ones evens out the end.  A chunk of 2048
@@ -256,10 +314,24 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     tiles_before = (uint32_t)(((uint64_t)want * tile_items + mixed - 1) / mixed);
     tiled = (uint32_t)(((uint64_t)(want + 1) * tile_items + mixed - 1) / mixed) > tiles_before;
   }
-  const uint32_t in_class = tiled ? tiles_before : want - tiles_before;
+  uint32_t in_class = tiled ? tiles_before : want - tiles_before;
+  // few rows: the item's bin, the longest first, and this thread's place in it
+  int32_t bin = -1;
+  uint32_t at_bin = 0;
+  if (sorted && !tiled) {
+#pragma unroll
+    for (int b = kBins - 1; b >= 0; --b) {
+      const uint32_t all = in_bin(all01, all23, b);
+      const bool here = bin < 0 && in_class < all;
+      in_class -= bin < 0 && !here ? all : 0;
+      at_bin = here ? in_bin(at01, at23, b) : at_bin;
+      bin = here ? b : bin;
+    }
+  }
   int32_t cut = 0;
   each([&](int32_t r, const Load& v) {
-    int32_t parts = parts_of(v);
+    const int32_t all = v.parts > 0 ? v.parts : parts_of(v);
+    int32_t parts = all;
     uint32_t cnt = (uint32_t)(v.tiles * parts);
     uint32_t& mine_at = v.tiled ? tile_at : few_at;
     const AttnClass& c = v.tiled ? a.tile : a.few;
@@ -275,13 +347,30 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       a.part_map[a.seqs + r] = parts;
       cut |= parts > 1;
     }
-    if (v.tiled == tiled && in_class - mine_at < cnt) {
-      const int32_t in = (int32_t)(in_class - mine_at);
-      // a chunk's last tokens have the most keys: its last tile comes first
-      const int32_t tile = v.tiled ? v.tiles - 1 - in / parts : in / parts, part = in % parts;
+    int32_t tile = -1, part = 0;
+    if (tiled || !sorted) {
+      const uint32_t in = in_class - mine_at;
+      if (v.tiled == tiled && in < cnt) {
+        tile = (int32_t)(in / (uint32_t)parts);
+        part = (int32_t)(in % (uint32_t)parts);
+        if (tiled) tile = v.tiles - 1 - tile;  // a chunk's last tokens have the most keys: first
+      }
+    } else if (!v.tiled) {
+      const uint32_t whole = whole_bin(all) == bin ? (uint32_t)(v.tiles * (all - 1)) : 0;
+      const uint32_t rest = rest_bin(v, all) == bin ? (uint32_t)v.tiles : 0;
+      const uint32_t in = in_class - at_bin;
+      if (cnt > 0 && in < whole) {
+        tile = (int32_t)(in / (uint32_t)(all - 1));
+        part = (int32_t)(in % (uint32_t)(all - 1));
+      } else if (cnt > 0 && in - whole < rest) {
+        tile = (int32_t)(in - whole);
+        part = all - 1;
+      }
+      at_bin += whole + rest;
+    }
+    if (tile >= 0)
       found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
                state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2), v.seq};
-    }
     mine_at += cnt;
   });
   if (map) {  // uniform over the workgroup

@@ -679,3 +679,33 @@ def test_chunks_of_long_heads(ops, dev, new, total, heads, kv_heads, head_size, 
     got, lse = call(ops, dev, b, return_lse=True, **kw)
     check(b, got, lse, reference(b, kw.get("causal", True), kw.get("window_left", -1)))
     assert torch.equal(call(ops, dev, b, **kw), got)
+
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,head_size,page,dtype,kw", [
+    # more items than the GPU takes at once, of all lengths: sorted into bins
+    ([1] * 70, [1 + (i * 619) % 2600 for i in range(70)], 16, 8, 64, 16, torch.bfloat16, {}),
+    ([1] * 150, [1 + (i * 619) % 1900 for i in range(150)], 8, 8, 64, 16, torch.float16, {}),
+    ([2] * 90, [2 + (i * 431) % 2100 for i in range(90)], 8, 8, 128, 32, torch.bfloat16, dict(window_left=1500)),
+    # beside a chunk
+    ([200, 1, 90] + [1] * 90, [700, 1500, 90] + [(i * 619) % 2300 for i in range(90)], 16, 8, 64, 16, torch.bfloat16, {}),
+    # several tiles per request (the hint of the second run is too small for them)
+    ([7] * 40, [7 + (i * 619) % 2400 for i in range(40)], 64, 16, 64, 16, torch.bfloat16, {}),
+])
+@pytest.mark.parametrize("hint", [None, 1])
+def test_ragged_batches_sorted_by_length(ops, dev, new, total, heads, kv_heads, head_size, page, dtype, kw, hint):
+    b = build_batch(44, page, new, total, heads, kv_heads, head_size, dtype)
+    got, lse = call(ops, dev, b, return_lse=True, max_query_len=hint, **kw)
+    check(b, got, lse, reference(b, True, kw.get("window_left", -1)))
+    assert torch.equal(call(ops, dev, b, max_query_len=hint, **kw), got)
+
+
+def test_windows_of_nothing_and_everything_and_large_pages(ops, dev):
+    for page in (4096, 48):
+        b = build_batch(45, page, [40, 1, 3], [300, 4500, 3], 8, 2, 64, torch.bfloat16, spare=1)
+        for window in (0, 1, 5000, 1 << 40):
+            got, lse = call(ops, dev, b, return_lse=True, window_left=window)
+            check(b, got, lse, reference(b, window=min(window, 1 << 20)))
+    d = to_dev(b, dev)                                  # a cache without a page: nobody sees a key
+    d["cache"] = d["cache"][:0]
+    out, lse = attend(ops, d, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
