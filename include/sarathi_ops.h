@@ -414,7 +414,8 @@ int sarathi_build_paged_kv_metadata(const int32_t* query_lens, const int32_t* se
  * kernel, and a wrong one costs time, not correctness.  workspace: scratch of
  * sarathi_paged_attention_workspace_bytes() bytes, 16-byte aligned, for the states of contexts that
  * are cut into parts to fill the GPU; contents irrelevant on entry and exit, not shared by calls
- * that may overlap.  With NULL or less nothing is cut (slower for few long contexts).
+ * that may overlap.  With NULL or less nothing is cut and nothing planned (slower for few long
+ * contexts and for more than 512 requests).
  */
 int64_t sarathi_paged_attention_workspace_bytes(int64_t num_tokens, int64_t num_seqs,
                                                 int64_t num_kv_indices, int num_heads,

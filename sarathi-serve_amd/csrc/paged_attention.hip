@@ -265,6 +265,13 @@ template <int DT> static int launch_join(const PagedAttnArgs& a, hipStream_t st)
   return launch_join_head<DT, 8>(a, st);
 }
 
+// ---- plans batches of many requests ---------------------------------------------------------------
+//
+// One workgroup, bound by latency: a run of requests per thread, three times over.
+__global__ __launch_bounds__(1024) void paged_attn_plan_kernel(PagedAttnArgs a) {
+  attn_find_item<16, true>(a, 0, a.part_map != nullptr);
+}
+
 // ---- what a call launches ------------------------------------------------------------------------
 
 // The requests of a batch fall into two classes by their rows (new tokens times query heads per key
@@ -273,9 +280,11 @@ struct AttnPlan {
   AttnClass few, tile;
   int64_t items;       // at most so many work items per key head, with contexts cut and without
   int64_t uncut_items;
-  int64_t map_bytes, ml_bytes, o_bytes;  // of the workspace; 0: nothing is cut
-  int64_t bytes() const { return map_bytes + ml_bytes + o_bytes; }
+  int64_t plan_bytes;                    // of the workspace; 0: workgroups look at all requests
+  int64_t map_bytes, ml_bytes, o_bytes;  // 0: nothing is cut
+  int64_t bytes() const { return plan_bytes + map_bytes + ml_bytes + o_bytes; }
 };
+constexpr int kPlanSeqs = 512;  // two per thread of a workgroup
 static int64_t round256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int log2_of(int v) {
   int n = 0;
@@ -341,6 +350,7 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   if (tiles > all_rows) tiles = all_rows;
   p.uncut_items = tiles;
   p.items = tiles + few_target + chunk_target;
+  if (seqs > kPlanSeqs) p.plan_bytes = round256((4 + 2 * seqs) * 4);
   const int64_t chunk_rows = p.tile.rows_log2 < 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
   const int64_t state_rows =
       chunk_rows + (p.few.rows_log2 < 0 ? 0 : ((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
@@ -468,12 +478,17 @@ extern "C" int sarathi_paged_attention(
       hipLaunchKernelGGL((paged_attn_plain_kernel<kF16>), grid, dim3(64), 0, st, a);
     return launch_status();
   }
-  // a workspace that is missing or too small means no cutting, not an error
-  const bool cut = p.bytes() > 0 && workspace && aligned16(workspace) && workspace_bytes >= p.bytes();
+  // a workspace that is missing or too small means no cutting and no plan, not an error
+  const bool have = workspace && aligned16(workspace) && workspace_bytes >= p.bytes();
+  const bool cut = have && p.map_bytes > 0;
   a.few = p.few;
   a.tile = p.tile;
+  char* w = reinterpret_cast<char*>(workspace);
+  if (have && p.plan_bytes > 0) {
+    a.plan = reinterpret_cast<uint32_t*>(w);
+    w += p.plan_bytes;
+  }
   if (cut) {
-    char* w = reinterpret_cast<char*>(workspace);
     a.part_map = reinterpret_cast<int32_t*>(w);
     a.part_ml = reinterpret_cast<float*>(w + p.map_bytes);
     a.part_o = reinterpret_cast<float*>(w + p.map_bytes + p.ml_bytes);
@@ -484,6 +499,10 @@ extern "C" int sarathi_paged_attention(
   if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
   // offsets inside a share of sixteen keys are 32-bit
   const bool page16 = page_size % 16 == 0 && a.entry_stride < (1 << 26);
+  if (a.plan) {
+    hipLaunchKernelGGL(paged_attn_plan_kernel, dim3(1), dim3(1024), 0, st, a);
+    if (const int rc = launch_status(); rc != SARATHI_OK) return rc;
+  }
   const int rc = launch_paged_attn(a, dtype, page16, groups, st);
   if (rc != SARATHI_OK || !cut) return rc;
   return dtype == kBF16 ? launch_join<kBF16>(a, st) : launch_join<kF16>(a, st);

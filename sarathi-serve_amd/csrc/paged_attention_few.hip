@@ -11,8 +11,7 @@ template <int DT, int DP, int RT, bool PAD, bool PAGE16>
 __global__ __launch_bounds__(64 * kAttnWaves) void paged_attn_few_kernel(PagedAttnArgs a) {
   extern __shared__ u32x4 few_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
-  const AttnItem it = attn_find_item(a, blockIdx.x / (uint32_t)a.kv_heads,
-                                     a.part_map != nullptr && blockIdx.x == 0);
+  const AttnItem it = attn_item(a, blockIdx.x / (uint32_t)a.kv_heads, blockIdx.x == 0);
   if (it.r < 0) return;
   few_item<DT, DP, RT, PAD, PAGE16>(a, it, h, (lds_char*)few_lds);
 }

@@ -50,6 +50,7 @@ struct PagedAttnArgs {
   float* part_o;          // states of the parts, or null: nothing is cut
   float* part_ml;         // [.. , 2]: reference (in powers of two) and sum
   int32_t* part_map;      // [seqs] first state row, [seqs] parts per tile, and whether any is cut
+  uint32_t* plan;         // or null: what the planning kernel found, see attn_planned_item
   int64_t q_stride, out_stride;           // elements
   int64_t page_stride, entry_stride;      // bytes
   uint32_t page_magic;    // ceil(2^page_shift / page_size): division of positions by page_size
@@ -141,22 +142,86 @@ SK_DEV int32_t attn_keys(const PagedAttnArgs& a, const AttnSeq& x) {
   return a.window >= 0 && s < x.s ? (int32_t)s : x.s;
 }
 
-// Finds item `want` of a key head: tiles of the chunks, in the order request, tile, part, and in between
-// those of few rows, sorted by length into kBins bins, the longest first, so that the end is even (256
-// requests: 5 % faster), unless they are short, all there at once, or so many (kSortRounds times what fills the GPU)
-// that the short ones in a row cost more (1000 requests: 4 % slower).  Two sums over the requests: keys times tiles of either class,
-// which fix the classes' part lengths, and the numbers of items.  A part is as long as filling the
-// GPU once allows but no longer than kPartKeys (below, its start and the way of its state to memory
-// and back weigh in), unless that made more than `target` items; it is at least min_part keys and a
-// multiple of 64.  Where no context is more than kCutKeys longer than that, nothing is cut: a workgroup
-// takes about 5 us for 512 keys, and joining parts as long.  When nothing is cut the first is left out.  The
-// workgroup with `map` set leaves the state rows for the kernel that joins the parts.  The work is
-// summed in 32-bit floats (it only chooses a length, the same in every workgroup; rounded up by more
-// than their error, so that the items stay within what the launch has workgroups for).
+SK_DEV AttnItem attn_uniform(const AttnItem& found) {  // the same in every lane: into scalar registers
+  AttnItem it;
+  it.r = __builtin_amdgcn_readfirstlane(found.r);
+  it.tiled = __builtin_amdgcn_readfirstlane(found.tiled);
+  it.tile = __builtin_amdgcn_readfirstlane(found.tile);
+  it.part = __builtin_amdgcn_readfirstlane(found.part);
+  it.parts = __builtin_amdgcn_readfirstlane(found.parts);
+  it.part_len = __builtin_amdgcn_readfirstlane(found.part_len);
+  it.state_row = __builtin_amdgcn_readfirstlane(found.state_row);
+  it.seq.q0 = __builtin_amdgcn_readfirstlane(found.seq.q0);
+  it.seq.n = __builtin_amdgcn_readfirstlane(found.seq.n);
+  it.seq.kv0 = __builtin_amdgcn_readfirstlane(found.seq.kv0);
+  it.seq.s = __builtin_amdgcn_readfirstlane(found.seq.s);
+  return it;
+}
+
+// Tiles of request r, and the keys that one spans; its parts once they are known.
+struct AttnLoad {
+  int32_t tiles, keys;
+  bool tiled;
+  AttnSeq seq;
+  int32_t parts;
+};
+SK_DEV AttnLoad attn_look(const PagedAttnArgs& a, int32_t r) {
+  const AttnSeq x = attn_seq(a, r);
+  const int64_t rows = (int64_t)x.n * a.group;
+  AttnLoad v;
+  v.tiled = a.few.rows_log2 < 0 || (a.tile.rows_log2 >= 0 && rows > a.few.max_rows);
+  const int32_t lg = v.tiled ? a.tile.rows_log2 : a.few.rows_log2;
+  v.tiles = (int32_t)((rows + ((int64_t)1 << lg) - 1) >> lg);
+  v.keys = attn_keys(a, x);
+  v.seq = x;
+  v.parts = 0;
+  return v;
+}
+SK_DEV int32_t attn_parts(int32_t keys, int32_t len) { return keys <= len ? 1 : (keys - 1) / len + 1; }
+// Index vectors that decrease can ask for more states than there are: such a request is left out.
+SK_DEV bool attn_no_room(const AttnClass& c, uint32_t before, int32_t tiles, int32_t parts) {
+  return parts > 1 && before + (uint64_t)tiles * (uint32_t)parts > (uint32_t)c.most;
+}
+SK_DEV int32_t attn_state_row(const PagedAttnArgs& a, const AttnClass& c, uint32_t item) {
+  return c.row_base + (int32_t)((item * (uint32_t)a.kv_heads) << c.rows_log2);
+}
+
+// Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
+// are at work all the time; the last quarter of the few ones evens out the end.  A chunk of 2048
+// tokens beside 256 decodes: 7 % faster than with all tiles first.
+SK_DEV bool attn_turn(uint32_t want, uint32_t tile_items, uint32_t few_items, uint32_t& in_class) {
+  const uint32_t mixed = tile_items + (uint32_t)((uint64_t)few_items * 3 / 4);
+  uint32_t tiles_before = tile_items;
+  bool tiled = false;
+  if (want < mixed) {
+    tiles_before = (uint32_t)(((uint64_t)want * tile_items + mixed - 1) / mixed);
+    tiled = (uint32_t)(((uint64_t)(want + 1) * tile_items + mixed - 1) / mixed) > tiles_before;
+  }
+  in_class = tiled ? tiles_before : want - tiles_before;
+  return tiled;
+}
+
+// Finds item `want` of a key head: tiles of the chunks, in the order request, tile, part, and in
+// between those of few rows, sorted by length into kBins bins, the longest first, so that the end is
+// even (256 requests: 5 % faster), unless they are short, all there at once, or so many (kSortRounds
+// times what fills the GPU) that the short ones in a row cost more (1000 requests: 4 % slower).
+//
+// Two sums over the requests: keys times tiles of either class, which fix the classes' part lengths,
+// and the numbers of items.  A part is as long as filling the GPU once allows but no longer than
+// kPartKeys (below, its start and the way of its state to memory and back weigh in), unless that
+// made more than `target` items; it is at least min_part keys and a multiple of 64.  Where no context
+// is more than kCutKeys longer than that, nothing is cut: a workgroup takes about 5 us for 512 keys,
+// and joining parts as long.  When nothing is cut the first sum is left out.  The workgroup with `map`
+// set leaves the state rows for the kernel that joins the parts.  The work is summed in 32-bit floats
+// (it only chooses a length, the same in every workgroup; rounded up by more than their error, so
+// that the items stay within what the launch has workgroups for).
+//
+// PLAN: one workgroup writes down what it finds for all requests instead (unsorted).
+template <int WAVES, bool PLAN>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
-  constexpr int WAVES = kAttnWaves;
   __shared__ float work_sums[2][2][WAVES];
-  __shared__ u32x4 sums[3];  // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3
+  // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3
+  __shared__ alignas(16) uint32_t sums[3][WAVES];
   __shared__ AttnItem found;
   constexpr int NT = WAVES * 64, KEEP = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -164,19 +229,8 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   const int64_t first = (int64_t)tid * run;
   const int32_t r0 = first < a.seqs ? (int32_t)first : a.seqs;
   const int32_t r1 = first + run < a.seqs ? (int32_t)(first + run) : a.seqs;
-  struct Load { int32_t tiles, keys; bool tiled; AttnSeq seq; int32_t parts; };
-  auto look = [&](int32_t r) {
-    const AttnSeq x = attn_seq(a, r);
-    const int64_t rows = (int64_t)x.n * a.group;
-    Load v;
-    v.tiled = a.few.rows_log2 < 0 || (a.tile.rows_log2 >= 0 && rows > a.few.max_rows);
-    const int32_t lg = v.tiled ? a.tile.rows_log2 : a.few.rows_log2;
-    v.tiles = (int32_t)((rows + ((int64_t)1 << lg) - 1) >> lg);
-    v.keys = attn_keys(a, x);
-    v.seq = x;
-    v.parts = 0;
-    return v;
-  };
+  typedef AttnLoad Load;
+  auto look = [&](int32_t r) { return attn_look(a, r); };
   Load kept[KEEP];  // the first requests of this thread are looked at once
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) {
@@ -239,7 +293,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       longest = fmaxf(longest, work_sums[0][1][w]);
     }
     const float len = fminf(longest, (float)(few_len >> 6));
-    sorted = __builtin_amdgcn_readfirstlane(
+    sorted = !PLAN && __builtin_amdgcn_readfirstlane(
         a.few.target > 0 && a.few.most <= 0xffff &&  // bins count in 16 bits
         longest > kPartKeys / 64 && work > len * (float)(a.few.fill - a.seqs) &&
         work <= len * (float)(kSortRounds * a.few.fill - a.seqs));
@@ -252,8 +306,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   // items in bin b of packed counts (those that are not sorted are one number, in the first word)
   auto in_bin = [](uint32_t c01, uint32_t c23, int b) { return ((b < 2 ? c01 : c23) >> (16 * (b & 1))) & 0xffffu; };
   auto parts_of = [&](const Load& v) {
-    const int32_t len = v.tiled ? tile_len : few_len;
-    return v.keys <= len ? 1 : (v.keys - 1) / len + 1;
+    return attn_parts(v.keys, v.tiled ? tile_len : few_len);
   };
   // the whole parts of a request of few rows, and the rest of each tile
   auto whole_bin = [&](int32_t parts) { return parts > 1 ? bin_of(few_len) : 0; };
@@ -276,45 +329,33 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   uint32_t tile_at = wave_scan(my_tile), at01 = wave_scan(my01), at23 = 0;
   if (sorted) at23 = wave_scan(my23);
   if (lane == 63) {
-    ((uint32_t*)&sums[0])[wave] = tile_at;
-    ((uint32_t*)&sums[1])[wave] = at01;
-    ((uint32_t*)&sums[2])[wave] = at23;
+    sums[0][wave] = tile_at;
+    sums[1][wave] = at01;
+    sums[2][wave] = at23;
   }
   tile_at -= my_tile;
   at01 -= my01;
   at23 -= my23;
   __syncthreads();
   uint32_t tile_items = 0, all01 = 0, all23 = 0;
-  {
-    const u32x4 t = sums[0], c = sums[1], d = sums[2];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) {
-        tile_at += t[w];
-        at01 += c[w];
-        at23 += d[w];
-      }
-      tile_items += t[w];
-      all01 += c[w];
-      all23 += d[w];
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) {
+      tile_at += sums[0][w];
+      at01 += sums[1][w];
+      at23 += sums[2][w];
     }
+    tile_items += sums[0][w];
+    all01 += sums[1][w];
+    all23 += sums[2][w];
   }
   uint32_t few_items = all01, few_at = at01;
   if (sorted) {
     few_items = (all01 & 0xffffu) + (all01 >> 16) + (all23 & 0xffffu) + (all23 >> 16);
     few_at = (at01 & 0xffffu) + (at01 >> 16) + (at23 & 0xffffu) + (at23 >> 16);
   }
-  // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
-  // are at work all the time; the last quarter of the few ones evens out the end.  A chunk of 2048
-  // tokens beside 256 decodes: 7 % faster than with all tiles first.
-  const uint32_t mixed = tile_items + (uint32_t)((uint64_t)few_items * 3 / 4);
-  uint32_t tiles_before = tile_items;
-  bool tiled = false;
-  if (want < mixed) {
-    tiles_before = (uint32_t)(((uint64_t)want * tile_items + mixed - 1) / mixed);
-    tiled = (uint32_t)(((uint64_t)(want + 1) * tile_items + mixed - 1) / mixed) > tiles_before;
-  }
-  uint32_t in_class = tiled ? tiles_before : want - tiles_before;
+  uint32_t in_class;
+  const bool tiled = attn_turn(want, tile_items, few_items, in_class);
   // few rows: the item's bin, the longest first, and this thread's place in it
   int32_t bin = -1;
   uint32_t at_bin = 0;
@@ -335,13 +376,16 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     uint32_t cnt = (uint32_t)(v.tiles * parts);
     uint32_t& mine_at = v.tiled ? tile_at : few_at;
     const AttnClass& c = v.tiled ? a.tile : a.few;
-    // index vectors that decrease can ask for more states than there are: such a request is left out
-    if (parts > 1 && mine_at + (uint64_t)v.tiles * (uint32_t)parts > (uint32_t)c.most) {
+    if (attn_no_room(c, mine_at, v.tiles, parts)) {
       mine_at += cnt;
       cnt = 0;
       parts = 1;
     }
-    const int32_t state = c.row_base + (int32_t)((mine_at * (uint32_t)a.kv_heads) << c.rows_log2);
+    if constexpr (PLAN) {
+      a.plan[4 + r] = few_at;
+      a.plan[4 + a.seqs + r] = tile_at;
+    }
+    const int32_t state = attn_state_row(a, c, mine_at);
     if (map) {
       a.part_map[r] = state;
       a.part_map[a.seqs + r] = parts;
@@ -368,29 +412,70 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       }
       at_bin += whole + rest;
     }
-    if (tile >= 0)
+    if (!PLAN && tile >= 0)
       found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
                state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2), v.seq};
     mine_at += cnt;
   });
+  if (PLAN && tid == 0) {
+    a.plan[0] = (uint32_t)few_len;
+    a.plan[1] = (uint32_t)tile_len;
+    a.plan[2] = few_items;
+    a.plan[3] = tile_items;
+  }
   if (map) {  // uniform over the workgroup
     cut = __syncthreads_or(cut);
     if (tid == 0) a.part_map[2 * a.seqs] = cut;
   }
   __syncthreads();
-  AttnItem it;
-  it.r = __builtin_amdgcn_readfirstlane(found.r);
-  it.tiled = __builtin_amdgcn_readfirstlane(found.tiled);
-  it.tile = __builtin_amdgcn_readfirstlane(found.tile);
-  it.part = __builtin_amdgcn_readfirstlane(found.part);
-  it.parts = __builtin_amdgcn_readfirstlane(found.parts);
-  it.part_len = __builtin_amdgcn_readfirstlane(found.part_len);
-  it.state_row = __builtin_amdgcn_readfirstlane(found.state_row);
-  it.seq.q0 = __builtin_amdgcn_readfirstlane(found.seq.q0);
-  it.seq.n = __builtin_amdgcn_readfirstlane(found.seq.n);
-  it.seq.kv0 = __builtin_amdgcn_readfirstlane(found.seq.kv0);
-  it.seq.s = __builtin_amdgcn_readfirstlane(found.seq.s);
+  return found;
+}
+
+// The same for batches of many requests, where looking at all of them in every workgroup would cost
+// more than a launch (2048 decodes of up to 300 keys: 0.90 ms, 0.34 this way): the planning kernel has left the part
+// lengths, the numbers of items and, for either class, the items before every request.
+SK_DEV AttnItem attn_planned_item(const PagedAttnArgs& a, uint32_t want) {
+  const int lane = threadIdx.x & 63;
+  AttnItem it = {};
+  it.r = -1;
+  uint32_t in_class;
+  const uint32_t few_items = a.plan[2], tile_items = a.plan[3];
+  const bool tiled = attn_turn(want, tile_items, few_items, in_class);
+  if (in_class >= (tiled ? tile_items : few_items)) return it;
+  const AttnClass& c = tiled ? a.tile : a.few;
+  const int32_t len = (int32_t)a.plan[tiled ? 1 : 0];
+  // the last request with no more items before it: 64 candidates at a time
+  const uint32_t* const before = a.plan + 4 + (tiled ? a.seqs : 0);
+  int32_t r = 0, width = a.seqs;
+  while (true) {
+    const int32_t step = (width + 63) / 64;
+    const bool ok = lane * step < width && before[r + lane * step] <= in_class;
+    const int cnt = __popcll(__builtin_amdgcn_ballot_w64(ok));
+    if (cnt == 0) return it;
+    r += (cnt - 1) * step;
+    if (step == 1) break;
+    width = width - (cnt - 1) * step < step ? width - (cnt - 1) * step : step;
+  }
+  r = __builtin_amdgcn_readfirstlane(r);
+  const AttnLoad v = attn_look(a, r);
+  const int32_t parts = attn_parts(v.keys, len);
+  const uint32_t first = before[r], in = in_class - first;
+  if (v.tiled != tiled || in >= (uint32_t)(v.tiles * parts) || attn_no_room(c, first, v.tiles, parts)) return it;
+  it.r = r;
+  it.tiled = tiled;
+  it.tile = (int32_t)(in / (uint32_t)parts);
+  it.part = (int32_t)(in % (uint32_t)parts);
+  if (tiled) it.tile = v.tiles - 1 - it.tile;
+  it.parts = parts;
+  it.part_len = len;
+  it.state_row = attn_state_row(a, c, first + (uint32_t)(it.tile * parts + it.part));
+  it.seq = v.seq;
   return it;
+}
+
+SK_DEV AttnItem attn_item(const PagedAttnArgs& a, uint32_t want, bool first) {
+  return attn_uniform(__builtin_expect(a.plan != nullptr, 0) ? attn_planned_item(a, want)
+                             : attn_find_item<kAttnWaves, false>(a, want, first && a.part_map != nullptr));
 }
 
 // Keys [begin, end) of a part; keys are counted from a multiple of 64, so that sixteen of them lie

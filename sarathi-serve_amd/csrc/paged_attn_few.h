@@ -13,10 +13,10 @@
 // Probabilities are rounded to the cache's type for the product (at most half a step each); maximum,
 // sum and output stay in 32 bits.
 //
-// Measured, bfloat16, 32 + 8 heads of 128, pages of 16: 256 requests of up to 8191 tokens (4.3 GB) 0.71 ms,
-// 6.05 TB/s, where a kernel that only reads the same way reaches 7.1; 64 such requests 0.20 ms, 5.5 TB/s;
-// one of 4096 tokens 10 us and 4 us more for the join.  With 256 requests two waves per workgroup took
-// 0.73 ms, eight 0.78, twice the stages with one workgroup per compute unit 0.81.
+// Measured, bfloat16, 32 + 8 heads of 128, pages of 16: 256 requests of up to 8191 tokens (4.3 GB) 0.68 ms,
+// 6.35 TB/s, where a kernel that only reads the same way reaches 7.1; 64 such requests 0.20 ms, 5.5 TB/s;
+// one of 4096 tokens 10 us and 4 us more for the join.  With 256 requests (0.715 ms then) two waves per
+// workgroup took 0.73 ms, eight 0.78, twice the stages with one workgroup per compute unit 0.81.
 #pragma once
 
 #include "paged_attn.h"

@@ -709,3 +709,45 @@ def test_windows_of_nothing_and_everything_and_large_pages(ops, dev):
     d["cache"] = d["cache"][:0]
     out, lse = attend(ops, d, return_lse=True)
     assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,head_size,page,dtype", [
+    ([1] * 700, [1 + (i * 619) % 150 for i in range(700)], 4, 2, 64, 16, torch.bfloat16),            # nothing to cut
+    ([1] * 699 + [1], [1 + (i * 619) % 150 for i in range(699)] + [4000], 4, 1, 64, 16, torch.float16),
+    ([i % 3 for i in range(1100)] + [170, 90], [(i * 37) % 90 for i in range(1100)] + [900, 1700], 8, 2, 64, 16,
+     torch.bfloat16),                                                                            # chunks and empty requests
+    ([0] * 513, [0] * 513, 4, 2, 64, 16, torch.bfloat16),
+])
+@pytest.mark.parametrize("hint", [None, 1])
+def test_batches_of_many_requests_are_planned(ops, dev, new, total, heads, kv_heads, head_size, page, dtype, hint):
+    """Above 512 requests a kernel plans the launch; without its workspace every workgroup looks at all."""
+    b = build_batch(46, page, new, total, heads, kv_heads, head_size, dtype)
+    want = reference(b)
+    got, lse = call(ops, dev, b, return_lse=True, max_query_len=hint)
+    check(b, got, lse, want)
+    if sum(new) == 0:
+        return
+    d, lib = to_dev(b, dev), abi.load()
+    out = torch.empty_like(d["query"])
+    abi.check(lib, _abi_attention(lib, d, out, abi.vp(None), 0, head_size ** -0.5, hint or 0))
+    check(b, out, None, want)
+
+
+def test_decreasing_index_vectors_stay_inside_a_planned_workspace(ops, dev):
+    lib = abi.load()
+    T, N, D, S = 64, 300, 64, 701
+    d = dict(query=torch.ones((T, 8, D), dtype=torch.bfloat16, device=dev),
+             cache=torch.ones((N, 2, 16, 1, D), dtype=torch.bfloat16, device=dev),
+             qo_indptr=torch.tensor([0, T] * ((S + 1) // 2), dtype=torch.int32, device=dev),
+             kv_indptr=torch.tensor([0, N] * ((S + 1) // 2), dtype=torch.int32, device=dev),
+             kv_indices=torch.arange(N, dtype=torch.int32, device=dev),
+             last=torch.full((S,), 16, dtype=torch.int32, device=dev))
+    need = lib.sarathi_paged_attention_workspace_bytes
+    need.restype = ctypes.c_int64
+    bytes_ = need(abi.i64(T), abi.i64(S), abi.i64(N), abi.ci(8), abi.ci(1), abi.ci(D), abi.ci(16), abi.i64(0))
+    guard = 1 << 24
+    ws = torch.full((bytes_ + 2 * guard,), 77, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(d["query"])
+    abi.check(lib, _abi_attention(lib, d, out, abi.vp(ws.data_ptr() + guard), bytes_, D ** -0.5))
+    torch.cuda.synchronize()
+    assert bool((ws[:guard] == 77).all()) and bool((ws[guard + bytes_:] == 77).all())
