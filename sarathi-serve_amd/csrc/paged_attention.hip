@@ -351,9 +351,10 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   p.uncut_items = tiles;
   p.items = tiles + few_target + chunk_target;
   if (seqs > kPlanSeqs) p.plan_bytes = round256((4 + 2 * seqs) * 4);
-  const int64_t chunk_rows = p.tile.rows_log2 < 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
+  // states of the classes that are cut
+  const int64_t chunk_rows = chunk_target == 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
   const int64_t state_rows =
-      chunk_rows + (p.few.rows_log2 < 0 ? 0 : ((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
+      chunk_rows + (few_target == 0 ? 0 : ((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
   if (few_target + chunk_target == 0 || state_rows >= 0x7fffffffLL) return p;
   p.few.target = (int32_t)few_target;
   p.tile.target = (int32_t)chunk_target;

@@ -59,6 +59,15 @@ def test_paged_attention_workspace(lib):
     assert size(2304, 257, 70000) < 1 << 30
 
 
+def test_paged_attention_workspace_of_large_chunks(lib):
+    """Chunks that fill the GPU are not cut: no room is asked for their states."""
+    f = lib.sarathi_paged_attention_workspace_bytes
+    f.restype = i64
+    small = f(i64(1 << 14), i64(2), i64(1 << 14), ci(32), ci(8), ci(128), ci(16), i64(0))
+    large = f(i64(1 << 17), i64(2), i64(1 << 14), ci(32), ci(8), ci(128), ci(16), i64(0))
+    assert 0 < large == small < 1 << 24
+
+
 def test_metadata_arguments(lib, p):
     def call(**k):
         g = k.get
