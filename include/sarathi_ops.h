@@ -311,10 +311,11 @@ int sarathi_moe_sum(void* out, const void* input, int64_t num_tokens, int64_t to
  * (flashinfer_attention_wrapper.py:262-273): token i's key and value rows are copied to entry
  * positions[i] % page_size of page kv_indices[kv_indptr[batch_indices[i]] + positions[i] /
  * page_size].  A token whose position, request or slot is negative goes nowhere (its cache stores
- * are dropped: the padding of a captured batch); otherwise indices are not range-checked.
+ * are dropped: the padding of a captured batch), and neither does one whose position lies past its
+ * request's pages [kv_indptr[b], kv_indptr[b + 1]); otherwise indices are not range-checked.
  *
  * sarathi_get_kv_slot_mapping (new) resolves that lookup once per batch:
- * slot_mapping[i] = page * page_size + entry.  The page table of a batch is the same for every
+ * slot_mapping[i] = page * page_size + entry, -1 where a token goes nowhere.  The page table of a batch is the same for every
  * layer, so the append entry points accept the vector in place of the four index arrays
  * (slot_mapping != NULL: batch_indices, positions, kv_indices and kv_indptr are ignored and may be
  * NULL) and then need one index load per token instead of three dependent ones.  The mapping is
@@ -374,7 +375,12 @@ int sarathi_rotary_embedding_append_paged_kv(
  *     0; a token whose index is negative (query_len > seq_len) or past its table row gets position
  *     and slot -1, one whose page number is negative slot -1.  The append entries skip both.
  * num_tokens and num_kv_pages are the lengths of those vectors, which the host knows; a larger
- * value leaves room for the batches of a captured graph.  page * page_size must stay below 2^31.
+ * value leaves room for the batches of a captured graph.  They have to hold the batch's new tokens
+ * and used pages.  Where they do not, nothing outside the vectors is touched, but the requests that
+ * do not fit are not served: their tokens past the pages that fit are appended by slot only (without
+ * slot_mapping they go nowhere), and attention sees such a request without the tokens and pages
+ * that were cut off, so its rows are not those of the whole sequence.
+ * page * page_size must stay below 2^31.
  */
 int sarathi_build_paged_kv_metadata(const int32_t* query_lens, const int32_t* seq_lens,
                                     const int32_t* block_tables, int32_t* qo_indptr,

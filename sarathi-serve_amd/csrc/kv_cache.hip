@@ -171,7 +171,12 @@ __global__ __launch_bounds__(256) void kv_slot_mapping_kernel(
   }
   const uint32_t pos = (uint32_t)positions[i];
   const uint32_t pg = pos / (uint32_t)page_size;
-  const int32_t page = kv_indices[(int64_t)kv_indptr[batch_indices[i]] + pg];
+  const int64_t b = batch_indices[i], first = kv_indptr[b], past = kv_indptr[b + 1];
+  if (first + pg >= past) {
+    slot_mapping[i] = -1;
+    return;
+  }
+  const int32_t page = kv_indices[first + pg];
   slot_mapping[i] = page * page_size + (int32_t)(pos - pg * (uint32_t)page_size);
 }
 

@@ -66,7 +66,9 @@ SK_DEV KvEntryKey kv_entry_key(const KvDest& d, int64_t tok) {
 }
 // SLOTS: whether k.a is a slot (known at compile time where a kernel is specialised on it).
 // Returns -1 for a token that goes nowhere: a negative slot, request or position (the rows behind
-// the last sequence of a padded batch).  Its stores are dropped; no table is looked up for it.
+// the last sequence of a padded batch), or a position past the pages that kv_indptr gives its request
+// (a batch whose pages outgrew kv_indices: what would be read next is another request's page, or none).
+// Its stores are dropped; no page is looked up for it.
 template <bool SLOTS>
 SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
   if (SLOTS) {
@@ -80,7 +82,9 @@ SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
   const uint32_t pos = (uint32_t)k.b;
   const uint32_t pg = pos / (uint32_t)d.page_size;
   const uint32_t entry = pos - pg * (uint32_t)d.page_size;
-  const int64_t page = d.kv_indices[(int64_t)d.kv_indptr[k.a] + pg];
+  const int64_t first = d.kv_indptr[k.a], past = d.kv_indptr[(int64_t)k.a + 1];
+  if (first + pg >= past) return -1;
+  const int64_t page = d.kv_indices[first + pg];
   return page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
 }
 SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {

@@ -50,7 +50,8 @@ def get_kv_slot_mapping(batch_indices: torch.Tensor, positions: torch.Tensor,
                         page_size: int) -> torch.Tensor:
     """``page * page_size + entry`` of every appended token.  The page table of a batch is the
     same for all layers: compute this once per batch and pass it as ``slot_mapping`` to the append
-    ops, which then resolve a token's destination with one index load instead of three."""
+    ops, which then resolve a token's destination with one index load instead of three.  -1 for a
+    token that goes nowhere: a negative request or position, or one past its request's pages."""
     slot_mapping = torch.empty_like(batch_indices)
     _C.get_kv_slot_mapping(batch_indices, positions, kv_indices, kv_indptr, slot_mapping, page_size)
     return slot_mapping
@@ -113,9 +114,12 @@ def build_paged_kv_metadata(query_lens: torch.Tensor, seq_lens: torch.Tensor,
     ``query_lens`` / ``seq_lens`` int32 ``[num_seqs]``: new tokens, and tokens in all after the
     append.  ``block_tables`` int32 ``[num_seqs, max_pages]``: each sequence's pages in order;
     entries past ``ceil(seq_len / page_size)`` are not read.  ``num_tokens`` and ``num_kv_pages``
-    (default: the size of ``block_tables``) are the lengths of the per-token vectors and of
-    ``kv_indices``; room beyond the batch, as a captured graph needs, is filled with -1
-    (``rope_positions``: 0), and the append ops skip negative slots and positions."""
+    (default: the size of ``block_tables``, which every batch fits) are the lengths of the per-token
+    vectors and of ``kv_indices``, and have to hold the batch's new tokens and used pages: requests that
+    do not fit are not served (nothing outside the vectors is touched, but attention sees them without
+    what was cut off, and their tokens past it are appended only by ``slot_mapping``).  Room beyond
+    the batch, as a captured graph needs, is filled with -1 (``rope_positions``: 0), and the append ops
+    skip negative slots and positions."""
     if num_kv_pages is None:
         num_kv_pages = block_tables.numel()
     return PagedKvMetadata._make(_C.build_paged_kv_metadata(query_lens, seq_lens, block_tables, page_size,

@@ -1,0 +1,80 @@
+"""GPU: what the paged-cache ops do at the limits of their arguments -- batches that outgrew their index
+vectors, index vectors that are no batch's, workspaces, padding and gradients."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import THETA_LLAMA3, cos_sin_cache, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(dev, v):
+    return torch.tensor(np.asarray(v), dtype=torch.int32, device=dev)
+
+
+# ---- more pages in use than kv_indices has room for ----------------------------------------------
+
+@pytest.mark.parametrize("room", [1, 4, 7, 8, 11])
+@pytest.mark.parametrize("fused", [False, True])
+def test_append_stays_within_the_pages_that_fit(ops, dev, room, fused):
+    """kv_indices is the front of a longer vector that goes on with pages which must not be written.  A
+    token whose page did not fit is not appended by the lookup; by slot it still lands in its table's page."""
+    page, heads, D = 4, 2, 64
+    new, total = [1, 9, 0, 5, 2], [8, 11, 3, 5, 14]                  # 2 + 3 + 1 + 2 + 4 pages
+    need = [-(-t // page) for t in total]
+    T, M = sum(new), 4
+    tables = torch.arange(5 * M, dtype=torch.int32).reshape(5, M).flip(1).to(dev)
+    f = ops.kv_cache_ops
+    m = f.build_paged_kv_metadata(i32(dev, new), i32(dev, total), tables, page, T, room)
+    assert m.kv_indptr.tolist() == np.minimum(np.concatenate([[0], np.cumsum(need)]), room).tolist()
+    longer = torch.full((room + 64,), 5 * M, dtype=torch.int32, device=dev)    # page 20 belongs to nobody
+    longer[:room] = m.kv_indices
+    ix = longer[:room]
+    g = gen(room)
+    qkv = randn((T, 6 * heads * D), g).to(dev)
+    cache = randn((5 * M + 1, 2, page, heads, D), g).to(dev)
+    q, k, v = qkv.split([4 * heads * D, heads * D, heads * D], dim=-1)
+    table = cos_sin_cache(64, D, THETA_LLAMA3, torch.bfloat16).to(dev)
+    if fused:                                                        # what the rotary embedding makes of the keys
+        wq, wk = q.clone(), k.clone()
+        ops.pos_encoding_ops.rotary_embedding(m.rope_positions, wq, wk, D, table, True)
+    else:
+        wk = k
+    fits, row = [], 0
+    want = cache.clone()
+    want_slots = cache.clone()
+    for r, (n, t) in enumerate(zip(new, total)):
+        own = min(max(room - sum(need[:r]), 0), need[r])
+        for j in range(n):
+            x = t - n + j
+            no = int(tables[r, x // page])
+            fits.append(no * page + x % page if x // page < own else -1)
+            for c in ([want] if fits[-1] >= 0 else []) + [want_slots]:
+                c[no, 0, x % page], c[no, 1, x % page] = wk[row].view(heads, D), v[row].view(heads, D)
+            row += 1
+    assert min(fits) < 0                                             # 12 pages are in use
+    got = f.get_kv_slot_mapping(m.batch_indices, m.positions, ix, m.kv_indptr, page)
+    assert got.tolist() == fits
+
+    def append(c, slots):
+        args = (m.batch_indices, m.positions, c, ix, m.kv_indptr)
+        if fused:
+            f.rotary_embedding_append_paged_kv(m.rope_positions, q.clone(), k.clone(), v, D, table, True, *args,
+                                               slot_mapping=slots)
+        else:
+            f.append_paged_kv_cache(k, v, *args, slot_mapping=slots)
+        return c
+    assert torch.equal(append(cache.clone(), None), want)
+    assert torch.equal(append(cache.clone(), got), want)
+    assert torch.equal(append(cache.clone(), m.slot_mapping), want_slots)
+    # heads whose rows are no multiple of 16 bytes: the element-wise kernel
+    if not fused:
+        small = torch.zeros((5 * M + 1, 2, page, heads, 3), dtype=torch.bfloat16, device=dev)
+        part = small.clone()
+        k3, v3 = k.view(T, heads, D)[..., :3].contiguous(), v.view(T, heads, D)[..., :3].contiguous()
+        f.append_paged_kv_cache(k3, v3, m.batch_indices, m.positions, part, ix, m.kv_indptr)
+        for row, s in enumerate(fits):
+            if s >= 0:
+                small[s // page, 0, s % page], small[s // page, 1, s % page] = k3[row], v3[row]
+        assert torch.equal(part, small)
