@@ -223,6 +223,9 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3
   __shared__ alignas(16) uint32_t sums[3][WAVES];
   __shared__ AttnItem found;
+  // Index vectors that decrease can overflow the packed counts below, and then more than one thread
+  // takes an item for its own: one of them may write it down, never a mixture of two requests.
+  __shared__ uint32_t taken;
   constexpr int NT = WAVES * 64, KEEP = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t run = (a.seqs + NT - 1) / NT;
@@ -246,7 +249,10 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       f(r, v);
     }
   };
-  if (tid == 0) found.r = -1;
+  if (tid == 0) {
+    found.r = -1;
+    taken = 0;
+  }
   int32_t few_len = 0x7fffffff, tile_len = 0x7fffffff;
   bool sorted = false;    // items of few rows, into bins
   float per_block = 0.f;  // bins per 64 keys
@@ -412,7 +418,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       }
       at_bin += whole + rest;
     }
-    if (!PLAN && tile >= 0)
+    if (!PLAN && tile >= 0 && atomicExch(&taken, 1u) == 0)
       found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
                state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2), v.seq};
     mine_at += cnt;

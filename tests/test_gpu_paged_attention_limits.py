@@ -78,3 +78,26 @@ def test_append_stays_within_the_pages_that_fit(ops, dev, room, fused):
             if s >= 0:
                 small[s // page, 0, s % page], small[s // page, 1, s % page] = k3[row], v3[row]
         assert torch.equal(part, small)
+
+
+# ---- index vectors that are no batch's --------------------------------------------------------------
+
+def test_items_that_more_than_one_request_claims(ops, dev):
+    """Index vectors that decrease, so that short requests name more tiles (over 100 000) than the item
+    search counts in 16 bits, beside one context that is cut and sorted: an item that several requests
+    claim is one request's, whole, and nothing in front of or behind `out` is written."""
+    T, H, D, N, S = 2048, 16, 64, 256, 300
+    qo = ([0, 1] + [500, T, 0, T] * S)[:S + 1]
+    kv = [0] + [N] * S
+    guard = 64
+    big = torch.full((T + 2 * guard, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    q = torch.ones((T, H, D), dtype=torch.bfloat16, device=dev)
+    cache = torch.ones((N, 2, 16, 2, D), dtype=torch.bfloat16, device=dev)
+    for _ in range(3):
+        out = ops.kv_cache_ops.paged_attention(
+            q, cache, i32(dev, qo), i32(dev, kv), torch.arange(N, dtype=torch.int32, device=dev),
+            torch.full((S,), 16, dtype=torch.int32, device=dev), out=big[guard:guard + T], max_query_len=1)
+        torch.cuda.synchronize()
+        assert bool((big[:guard] == 7).all()) and bool((big[guard + T:] == 7).all())
+        # values are all 1: a row is a mean of ones, 0 (a request without keys) or as it was
+        assert bool(((out == 1) | (out == 0) | (out == 7)).all())
