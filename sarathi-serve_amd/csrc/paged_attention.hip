@@ -278,6 +278,7 @@ __global__ __launch_bounds__(1024) void paged_attn_plan_kernel(PagedAttnArgs a) 
 // head): few rows, and chunks, which are taken in large tiles.  All sizes here are known on the host.
 struct AttnPlan {
   AttnClass few, tile;
+  int64_t state_room;  // rows of states per key head
   int64_t items;       // at most so many work items per key head, with contexts cut and without
   int64_t uncut_items;
   int64_t plan_bytes;                    // of the workspace; 0: workgroups look at all requests
@@ -351,16 +352,17 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   p.uncut_items = tiles;
   p.items = tiles + few_target + chunk_target;
   if (seqs > kPlanSeqs) p.plan_bytes = round256((4 + 2 * seqs) * 4);
-  // states of the classes that are cut
-  const int64_t chunk_rows = chunk_target == 0 ? 0 : ((chunk_tiles + chunk_target) * kv_heads) << p.tile.rows_log2;
-  const int64_t state_rows =
-      chunk_rows + (few_target == 0 ? 0 : ((few_tiles + few_target) * kv_heads) << p.few.rows_log2);
+  // Only cut tiles leave states.  All cuts together add at most `target` parts and every cut tile has at
+  // least one of them, so no more than `target` tiles are cut.
+  auto states = [](int64_t tiles, int64_t target, const AttnClass& c) {
+    return target == 0 ? 0 : ((tiles < target ? tiles : target) + target) << c.rows_log2;
+  };
+  p.state_room = states(few_tiles, few_target, p.few) + states(chunk_tiles, chunk_target, p.tile);
+  const int64_t state_rows = p.state_room * kv_heads;
   if (few_target + chunk_target == 0 || state_rows >= 0x7fffffffLL) return p;
   p.few.target = (int32_t)few_target;
   p.tile.target = (int32_t)chunk_target;
-  p.few.row_base = (int32_t)chunk_rows;
   p.few.most = (int32_t)(few_tiles + few_target);
-  p.tile.most = (int32_t)(chunk_tiles + chunk_target);
   p.map_bytes = round256((2 * seqs + 1) * 4);
   p.ml_bytes = round256(state_rows * 8);
   p.o_bytes = round256(state_rows * head_size * 4);
@@ -493,6 +495,7 @@ extern "C" int sarathi_paged_attention(
     a.part_map = reinterpret_cast<int32_t*>(w);
     a.part_ml = reinterpret_cast<float*>(w + p.map_bytes);
     a.part_o = reinterpret_cast<float*>(w + p.map_bytes + p.ml_bytes);
+    a.state_room = (int32_t)p.state_room;
   } else {
     a.few.target = a.tile.target = 0;
   }

@@ -33,8 +33,7 @@ struct AttnClass {
   int32_t target;     // items per key head that cutting stays below; 0: do not cut
   int32_t fill;       // items per key head that fill the GPU once
   int32_t min_part;   // least keys of a part, a multiple of 64
-  int32_t row_base;   // first state row of the class
-  int32_t most;       // items there is room for in the states; sound index vectors stay within
+  int32_t most;       // few: items that sound index vectors stay within, cut or not
 };
 
 struct PagedAttnArgs {
@@ -50,6 +49,7 @@ struct PagedAttnArgs {
   float* part_o;          // states of the parts, or null: nothing is cut
   float* part_ml;         // [.. , 2]: reference (in powers of two) and sum
   int32_t* part_map;      // [seqs] first state row, [seqs] parts per tile, and whether any is cut
+  int32_t state_room;     // rows per key head that there is room for in the states
   uint32_t* plan;         // or null: what the planning kernel found, see attn_planned_item
   int64_t q_stride, out_stride;           // elements
   int64_t page_stride, entry_stride;      // bytes
@@ -117,7 +117,7 @@ struct AttnItem {
   int32_t tiled;     // 1: a tile of a chunk, 0: a tile of few rows
   int32_t tile;      // tile of its rows
   int32_t part, parts, part_len;
-  int32_t state_row; // first state row of this tile and part (key head 0)
+  int32_t state_row; // first state row of this tile and part (key head 0), where parts > 1
   AttnSeq seq;
 };
 
@@ -178,12 +178,17 @@ SK_DEV AttnLoad attn_look(const PagedAttnArgs& a, int32_t r) {
   return v;
 }
 SK_DEV int32_t attn_parts(int32_t keys, int32_t len) { return keys <= len ? 1 : (keys - 1) / len + 1; }
-// Index vectors that decrease can ask for more states than there are: such a request is left out.
-SK_DEV bool attn_no_room(const AttnClass& c, uint32_t before, int32_t tiles, int32_t parts) {
-  return parts > 1 && before + (uint64_t)tiles * (uint32_t)parts > (uint32_t)c.most;
+// States are kept of cut requests only, both classes' in one row: the rows per key head that a request
+// needs for its states.
+SK_DEV uint32_t attn_state_rows(const AttnClass& c, int32_t tiles, int32_t parts) {
+  return parts > 1 ? ((uint32_t)tiles * (uint32_t)parts) << c.rows_log2 : 0;
 }
-SK_DEV int32_t attn_state_row(const PagedAttnArgs& a, const AttnClass& c, uint32_t item) {
-  return c.row_base + (int32_t)((item * (uint32_t)a.kv_heads) << c.rows_log2);
+// Index vectors that decrease can ask for more states than there are: such a request is left out.
+SK_DEV bool attn_no_room(const PagedAttnArgs& a, const AttnClass& c, uint32_t before, int32_t tiles, int32_t parts) {
+  return parts > 1 && before + (((uint64_t)tiles * (uint32_t)parts) << c.rows_log2) > (uint32_t)a.state_room;
+}
+SK_DEV int32_t attn_state_at(const PagedAttnArgs& a, const AttnClass& c, int32_t first, int32_t item) {
+  return first + (int32_t)((uint32_t)(item * a.kv_heads) << c.rows_log2);
 }
 
 // Tiles of chunks (bound by the matrix cores) and of few rows (by memory) in turn, so that both
@@ -220,8 +225,8 @@ SK_DEV bool attn_turn(uint32_t want, uint32_t tile_items, uint32_t few_items, ui
 template <int WAVES, bool PLAN>
 SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) {
   __shared__ float work_sums[2][2][WAVES];
-  // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3
-  __shared__ alignas(16) uint32_t sums[3][WAVES];
+  // of the waves: items of chunks, of few rows in bins 0 and 1, 2 and 3; rows of the states
+  __shared__ alignas(16) uint32_t sums[4][WAVES];
   __shared__ AttnItem found;
   // Index vectors that decrease can overflow the packed counts below, and then more than one thread
   // takes an item for its own: one of them may write it down, never a mixture of two requests.
@@ -319,10 +324,12 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
   auto rest_bin = [&](const Load& v, int32_t parts) {
     return bin_of(parts > 1 ? v.keys - (parts - 1) * few_len : v.keys);
   };
-  uint32_t my_tile = 0, my01 = 0, my23 = 0;
+  const bool cutting = (few_len & tile_len) != 0x7fffffff;
+  uint32_t my_tile = 0, my01 = 0, my23 = 0, my_state = 0;
   auto add = [&](int32_t b, uint32_t n) { (b < 2 ? my01 : my23) += n << (16 * (b & 1)); };
   each([&](int32_t, Load& v) {
     v.parts = parts_of(v);
+    my_state += attn_state_rows(v.tiled ? a.tile : a.few, v.tiles, v.parts);
     if (v.tiled) {
       my_tile += (uint32_t)(v.tiles * v.parts);
     } else if (sorted) {
@@ -332,16 +339,19 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       my01 += (uint32_t)(v.tiles * v.parts);
     }
   });
-  uint32_t tile_at = wave_scan(my_tile), at01 = wave_scan(my01), at23 = 0;
+  uint32_t tile_at = wave_scan(my_tile), at01 = wave_scan(my01), at23 = 0, state_at = 0;
   if (sorted) at23 = wave_scan(my23);
+  if (cutting) state_at = wave_scan(my_state);
   if (lane == 63) {
     sums[0][wave] = tile_at;
     sums[1][wave] = at01;
     sums[2][wave] = at23;
+    sums[3][wave] = state_at;
   }
   tile_at -= my_tile;
   at01 -= my01;
   at23 -= my23;
+  state_at -= my_state;
   __syncthreads();
   uint32_t tile_items = 0, all01 = 0, all23 = 0;
 #pragma unroll
@@ -350,6 +360,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
       tile_at += sums[0][w];
       at01 += sums[1][w];
       at23 += sums[2][w];
+      state_at += sums[3][w];
     }
     tile_items += sums[0][w];
     all01 += sums[1][w];
@@ -382,16 +393,17 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     uint32_t cnt = (uint32_t)(v.tiles * parts);
     uint32_t& mine_at = v.tiled ? tile_at : few_at;
     const AttnClass& c = v.tiled ? a.tile : a.few;
-    if (attn_no_room(c, mine_at, v.tiles, parts)) {
+    const int32_t state = (int32_t)(state_at * (uint32_t)a.kv_heads);
+    if (attn_no_room(a, c, state_at, v.tiles, parts)) {
       mine_at += cnt;
       cnt = 0;
       parts = 1;
     }
+    state_at += attn_state_rows(c, v.tiles, all);
     if constexpr (PLAN) {
       a.plan[4 + r] = few_at;
       a.plan[4 + a.seqs + r] = tile_at;
     }
-    const int32_t state = attn_state_row(a, c, mine_at);
     if (map) {
       a.part_map[r] = state;
       a.part_map[a.seqs + r] = parts;
@@ -420,7 +432,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
     }
     if (!PLAN && tile >= 0 && atomicExch(&taken, 1u) == 0)
       found = {r, v.tiled, tile, part, parts, v.tiled ? tile_len : few_len,
-               state + (int32_t)((uint32_t)((tile * parts + part) * a.kv_heads) << c.rows_log2), v.seq};
+               attn_state_at(a, c, state, tile * parts + part), v.seq};
     mine_at += cnt;
   });
   if (PLAN && tid == 0) {
@@ -439,7 +451,7 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
 
 // The same for batches of many requests, where looking at all of them in every workgroup would cost
 // more than a launch (2048 decodes of up to 300 keys: 0.90 ms, 0.34 this way): the planning kernel has left the part
-// lengths, the numbers of items and, for either class, the items before every request.
+// lengths, the numbers of items, for either class the items before every request, and the state rows.
 SK_DEV AttnItem attn_planned_item(const PagedAttnArgs& a, uint32_t want) {
   const int lane = threadIdx.x & 63;
   AttnItem it = {};
@@ -466,7 +478,8 @@ SK_DEV AttnItem attn_planned_item(const PagedAttnArgs& a, uint32_t want) {
   const AttnLoad v = attn_look(a, r);
   const int32_t parts = attn_parts(v.keys, len);
   const uint32_t first = before[r], in = in_class - first;
-  if (v.tiled != tiled || in >= (uint32_t)(v.tiles * parts) || attn_no_room(c, first, v.tiles, parts)) return it;
+  if (v.tiled != tiled || in >= (uint32_t)(v.tiles * parts)) return it;
+  if (parts > 1 && a.part_map[a.seqs + r] != parts) return it;  // no room for its states
   it.r = r;
   it.tiled = tiled;
   it.tile = (int32_t)(in / (uint32_t)parts);
@@ -474,7 +487,7 @@ SK_DEV AttnItem attn_planned_item(const PagedAttnArgs& a, uint32_t want) {
   if (tiled) it.tile = v.tiles - 1 - it.tile;
   it.parts = parts;
   it.part_len = len;
-  it.state_row = attn_state_row(a, c, first + (uint32_t)(it.tile * parts + it.part));
+  it.state_row = parts > 1 ? attn_state_at(a, c, a.part_map[r], it.tile * parts + it.part) : 0;
   it.seq = v.seq;
   return it;
 }

@@ -1,10 +1,15 @@
 """GPU: what the paged-cache ops do at the limits of their arguments -- batches that outgrew their index
 vectors, index vectors that are no batch's, workspaces, padding and gradients."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
+import abi_ctypes as abi
 from helpers import THETA_LLAMA3, cos_sin_cache, gen, randn
+from test_gpu_paged_attention import build_batch, check, reference
+from test_gpu_paged_attention_use import _abi_attention, attend, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +106,35 @@ def test_items_that_more_than_one_request_claims(ops, dev):
         assert bool((big[:guard] == 7).all()) and bool((big[guard + T:] == 7).all())
         # values are all 1: a row is a mean of ones, 0 (a request without keys) or as it was
         assert bool(((out == 1) | (out == 0) | (out == 7)).all())
+
+
+# ---- states of cut contexts -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("new,total,heads,kv_heads,hint", [
+    # cut decodes in front of, between and behind uncut ones
+    ([1] * 40, [3000 if i % 13 == 0 else 30 + i for i in range(40)], 8, 2, 1),
+    ([1] * 40, [3000 if i % 13 == 5 else 30 + i for i in range(40)], 8, 2, 0),
+    # cut chunks and cut decodes in turn, empty requests
+    ([70, 1, 0, 33, 1, 1, 64], [4200, 2900, 0, 90, 5000, 7, 3100], 8, 2, 0),
+    # the same above 512 requests, where a kernel plans the launch
+    ([1] * 600, [2500 if i % 97 == 0 else 1 + i % 50 for i in range(600)], 4, 2, 1),
+    ([1] * 300 + [50] + [1] * 300 + [41], [1 + i % 50 for i in range(300)] + [3500] + [2100] + [9] * 299 + [2600], 8, 2, 0),
+])
+def test_states_of_cut_contexts_among_uncut_ones(ops, dev, new, total, heads, kv_heads, hint):
+    """Only cut requests have states, and they fit the workspace asked for."""
+    b = build_batch(50, 16, new, total, heads, kv_heads, 64, torch.bfloat16)
+    d, lib = to_dev(b, dev), abi.load()
+    need = lib.sarathi_paged_attention_workspace_bytes
+    need.restype = ctypes.c_int64
+    bytes_ = need(abi.i64(sum(new)), abi.i64(len(new)), abi.i64(d["kv_indices"].numel()), abi.ci(heads), abi.ci(kv_heads),
+                  abi.ci(64), abi.ci(16), abi.i64(hint))
+    assert bytes_ > 0
+    guard = 1 << 20
+    ws = torch.full((bytes_ + 2 * guard,), 77, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(d["query"])
+    abi.check(lib, _abi_attention(lib, d, out, abi.vp(ws.data_ptr() + guard), bytes_, 64 ** -0.5, hint))
+    check(b, out, None, reference(b))
+    assert bool((ws[:guard] == 77).all()) and bool((ws[guard + bytes_:] == 77).all())
+    # and through the front end, twice: nothing depends on the order of workgroups
+    for _ in range(2):
+        assert torch.equal(attend(ops, d, max_query_len=hint), out)

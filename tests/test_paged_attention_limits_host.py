@@ -1,0 +1,32 @@
+"""Sizes and refusals of the paged-cache ops that need no GPU."""
+import ctypes
+import os
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+LIB = os.path.join(ROOT, "sarathi-serve_amd", "sarathi_amd", "lib", "libsarathi_ops_hip.so")
+i64, ci = ctypes.c_int64, ctypes.c_int
+
+
+@pytest.fixture(scope="module")
+def workspace():
+    import sarathi_amd  # noqa: F401  loads torch first
+    f = ctypes.CDLL(LIB).sarathi_paged_attention_workspace_bytes
+    f.restype = i64
+    return lambda T, R, NI, h, hk, d, page, q: f(i64(T), i64(R), i64(NI), ci(h), ci(hk), ci(d), ci(page), i64(q))
+
+
+@pytest.mark.parametrize("h,hk,d", [(32, 8, 128), (32, 32, 128), (64, 64, 128), (64, 8, 128), (71, 1, 64), (12, 4, 256)])
+@pytest.mark.parametrize("hint", [0, 1])
+def test_workspace_does_not_grow_with_requests_that_are_not_cut(workspace, h, hk, d, hint):
+    """Every cut adds parts, of which there are at most four times what fills the GPU (two workgroups per
+    compute unit, shared by the key heads, 256 units), and cuts no more tiles than it adds parts.  So the
+    states take at most 2 * 4 * 512 tiles of 64 rows of d + 2 floats and the chunks' at most 2 * 512 of 128
+    rows, whatever the number of requests; their maps and the plan take 16 bytes a request."""
+    states = (2 * 4 * 512 * 64 + 2 * 512 * 128) * (d + 2) * 4
+    if hint == 1:      # tiles of 16, 32 or 64 rows, by the query heads per key head; no chunks
+        states = 2 * 4 * 512 * (16 if h // hk <= 16 else 64) * (d + 2) * 4
+    for R in (1, 16, 300, 600, 4096, 8192, 65536):
+        size = workspace(R, R, 64 * R, h, hk, d, 16, hint)
+        assert 0 < size <= states + 16 * R + 8192, (R, size)
