@@ -57,6 +57,12 @@ void check_gpu(const torch::Tensor& t, const torch::Tensor& like, const char* op
               " but the first tensor is on ", like.device());
 }
 
+// For ops that return new tensors: these carry no graph, so a gradient asked for would be lost in silence.
+void check_no_grad(const torch::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), op, ": ", name,
+              " requires a gradient, which is not computed; detach it or call under torch.no_grad()");
+}
+
 // Makes `dev` the current HIP device for the scope and yields torch's current
 // stream on it.
 struct LaunchScope {
@@ -475,6 +481,10 @@ std::vector<torch::Tensor> paged_attention(
   check_i32(kv_indptr, query, op, "kv_indptr");
   check_i32(kv_indices, query, op, "kv_indices");
   check_i32(kv_last_page_len, query, op, "kv_last_page_len");
+  check_no_grad(query, op, "query");
+  check_no_grad(cache, op, v_cache.has_value() ? "k_cache" : "paged_kv_cache");
+  if (v_cache.has_value()) check_no_grad(*v_cache, op, "v_cache");
+  if (out_or_none.has_value()) check_no_grad(*out_or_none, op, "out");
   TORCH_CHECK(query.scalar_type() == at::ScalarType::Half ||
                   query.scalar_type() == at::ScalarType::BFloat16,
               op, ": only bfloat16 and float16 are supported, got ", query.scalar_type());
@@ -552,6 +562,8 @@ std::vector<torch::Tensor> merge_attention_states(const torch::Tensor& v, const 
   const char* op = "merge_attention_states";
   check_gpu(v, v, op, "v");
   check_gpu(lse, v, op, "lse");
+  check_no_grad(v, op, "v");
+  check_no_grad(lse, op, "lse");
   const int code = dtype_code(v, op);
   TORCH_CHECK(v.dim() == 4 && lse.dim() == 3 && lse.size(0) == v.size(0) && lse.size(1) == v.size(1) &&
                   lse.size(2) == v.size(2),

@@ -146,7 +146,8 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: 
     Returns ``out`` (shaped like ``query``), with ``return_lse`` also the natural-log sums
     ``[num_tokens, num_heads]`` (float32) that ``merge_attention_states`` joins.  A token that sees no
     key gets 0 and -inf; rows behind the last request are not written.  ``out`` must not overlap
-    ``query`` or the cache.  A value that a mask hides from some of a request's tokens only must be finite."""
+    ``query`` or the cache.  A value that a mask hides from some of a request's tokens only must be finite.
+    No gradients: inputs that require one are refused unless gradients are switched off."""
     if kv_layout != "NHD":
         raise ValueError("only the NHD page layout is supported, got %r" % (kv_layout,))
     if isinstance(paged_kv_cache, (tuple, list)):
@@ -163,7 +164,8 @@ def merge_attention_states(v: torch.Tensor, lse: torch.Tensor) -> Tuple[torch.Te
     """Joins ``paged_attention`` states over disjoint parts of a context, e.g. a prefix that requests
     share and each request's own suffix: ``v`` ``[states, tokens, heads, head_size]``, ``lse``
     ``[states, tokens, heads]`` (natural log, float32).  The state and token dimensions may have any
-    strides.  Returns the joined output and its lse; states with lse -inf are left out."""
+    strides.  Returns the joined output and its lse; states with lse -inf are left out.  No gradients:
+    inputs that require one are refused unless gradients are switched off."""
     out, out_lse = _C.merge_attention_states(v, lse)
     return out, out_lse
 

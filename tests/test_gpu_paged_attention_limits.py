@@ -138,3 +138,35 @@ def test_states_of_cut_contexts_among_uncut_ones(ops, dev, new, total, heads, kv
     # and through the front end, twice: nothing depends on the order of workgroups
     for _ in range(2):
         assert torch.equal(attend(ops, d, max_query_len=hint), out)
+
+
+# ---- gradients --------------------------------------------------------------------------------------
+
+def test_inputs_that_require_a_gradient_are_refused(ops, dev):
+    """Nothing is differentiated here, and results without a graph would drop the gradient in silence."""
+    b = build_batch(51, 16, [3, 1], [40, 9], 4, 2, 64, torch.bfloat16, poison=False)
+    d = to_dev(b, dev)
+    f, merge = ops.kv_cache_ops.paged_attention, ops.kv_cache_ops.merge_attention_states
+    index = (d["qo_indptr"], d["kv_indptr"], d["kv_indices"], d["last"])
+    want, lse = attend(ops, d, return_lse=True)
+    kc, vc = d["cache"][:, 0].contiguous(), d["cache"][:, 1].contiguous()
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for args, kw, name in (((grad(d["query"]), d["cache"]), {}, "query"), ((d["query"], grad(d["cache"])), {}, "paged_kv_cache"),
+                           ((d["query"], (grad(kc), vc)), {}, "k_cache"), ((d["query"], (kc, grad(vc))), {}, "v_cache"),
+                           ((d["query"], d["cache"]), dict(out=grad(want)), "out")):
+        with pytest.raises(RuntimeError, match=name + " requires a gradient"):
+            f(*args, *index, **kw)
+        with torch.no_grad():
+            assert torch.equal(f(*args, *index, **kw), want)
+        with torch.inference_mode():
+            if "out" not in kw:
+                assert torch.equal(f(*args, *index, **kw), want)
+    # a value that was computed from a parameter, not a leaf
+    with pytest.raises(RuntimeError, match="query requires a gradient"):
+        f(grad(d["query"]) * 1.0, d["cache"], *index)
+    v, z = torch.stack((want, want)), torch.stack((lse, lse))
+    for args, name in (((grad(v), z), "v"), ((v, grad(z)), "lse")):
+        with pytest.raises(RuntimeError, match=name + " requires a gradient"):
+            merge(*args)
+        with torch.no_grad():
+            assert torch.equal(merge(*args)[0], want)
