@@ -436,6 +436,18 @@ int sarathi_paged_attention(const void* query, const void* k_cache, const void* 
                             int64_t page_stride, int64_t entry_stride, float sm_scale, int causal,
                             int64_t window_left, int64_t max_query_len, void* workspace,
                             int64_t workspace_bytes, int dtype, void* stream);
+/* The same for a caller whose out or lse are new memory: fill_rows says what the rows outside
+ * [qo_indptr[0], qo_indptr[num_seqs]) become instead of being left as they were: bit 0: lse = -inf
+ * (where lse is not NULL), bit 1: out = 0.  num_seqs = 0 leaves rows of no other kind. */
+int sarathi_paged_attention_fill(const void* query, const void* k_cache, const void* v_cache, void* out,
+                                 float* lse, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                 const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                 int64_t num_tokens, int64_t num_seqs, int64_t num_kv_indices,
+                                 int64_t num_pages, int num_heads, int num_kv_heads, int head_size,
+                                 int page_size, int64_t query_stride, int64_t out_stride,
+                                 int64_t page_stride, int64_t entry_stride, float sm_scale, int causal,
+                                 int64_t window_left, int64_t max_query_len, void* workspace,
+                                 int64_t workspace_bytes, int dtype, int fill_rows, void* stream);
 
 /*
  * New entry: joins attention states computed over disjoint parts of a context (e.g. a prefix that

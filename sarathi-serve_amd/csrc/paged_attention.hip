@@ -24,7 +24,13 @@ __global__ __launch_bounds__(64) void paged_attn_plain_kernel(PagedAttnArgs a) {
   __shared__ float prob[64];
   const int lane = threadIdx.x;
   const int32_t tok = (int32_t)blockIdx.x, head = (int32_t)blockIdx.y;
-  if (tok >= clamp_i32(a.qo_indptr[a.seqs], 0, a.tokens) || tok < a.qo_indptr[0]) return;
+  if (a.seqs == 0 || tok >= clamp_i32(a.qo_indptr[a.seqs], 0, a.tokens) || tok < a.qo_indptr[0]) {
+    const int64_t row = (int64_t)tok * a.out_stride + (int64_t)head * a.head_size;
+    if (a.fill & 2)
+      for (int d = lane; d < a.head_size; d += 64) store_elem<DT>(a.out, row + d, 0.f);
+    if ((a.fill & 1) && lane == 0) a.lse[(int64_t)tok * a.heads + head] = -INFINITY;
+    return;
+  }
   int32_t lo_r = 0, hi_r = a.seqs;
   while (hi_r - lo_r > 1) {
     const int32_t mid = (lo_r + hi_r) >> 1;
@@ -285,7 +291,8 @@ struct AttnPlan {
   int64_t map_bytes, ml_bytes, o_bytes;  // 0: nothing is cut
   int64_t bytes() const { return plan_bytes + map_bytes + ml_bytes + o_bytes; }
 };
-constexpr int kPlanSeqs = 512;  // two per thread of a workgroup
+constexpr int kPlanSeqs = 512;   // two per thread of a workgroup
+constexpr int kFillGroups = 64;  // workgroups that fill the rows of no request
 static int64_t round256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int log2_of(int v) {
   int n = 0;
@@ -411,14 +418,15 @@ extern "C" int64_t sarathi_paged_attention_workspace_bytes(int64_t num_tokens, i
   return p.bytes();
 }
 
-extern "C" int sarathi_paged_attention(
+extern "C" int sarathi_paged_attention_fill(
     const void* query, const void* k_cache, const void* v_cache, void* out, float* lse,
     const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
     const int32_t* kv_last_page_len, int64_t num_tokens, int64_t num_seqs, int64_t num_kv_indices,
     int64_t num_pages, int num_heads, int num_kv_heads, int head_size, int page_size,
     int64_t query_stride, int64_t out_stride, int64_t page_stride, int64_t entry_stride,
     float sm_scale, int causal, int64_t window_left, int64_t max_query_len, void* workspace,
-    int64_t workspace_bytes, int dtype, void* stream) {
+    int64_t workspace_bytes, int dtype, int fill_rows, void* stream) {
+  if (fill_rows < 0 || fill_rows > 3) return SARATHI_ERR_INVALID_ARG;
   if (!attn_sizes_ok(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads, head_size,
                      page_size) || num_pages < 0)
     return SARATHI_ERR_INVALID_ARG;
@@ -436,7 +444,9 @@ extern "C" int sarathi_paged_attention(
       !attn_sizes_fit(num_tokens, num_seqs, num_kv_indices, num_heads, head_size) ||
       num_pages >= 0x7fffffffLL)
     return SARATHI_ERR_UNSUPPORTED;
-  if (num_tokens == 0 || num_seqs == 0) return SARATHI_OK;
+  const int fill = lse ? fill_rows : fill_rows & 2;
+  if (num_tokens == 0 || (num_seqs == 0 && fill == 0)) return SARATHI_OK;
+  if (num_seqs == 0 && (fill & 2) && !out) return SARATHI_ERR_INVALID_ARG;
   const AttnPlan p = plan_attention(num_tokens, num_seqs, num_kv_indices, num_heads, num_kv_heads,
                               head_size, page_size, max_query_len);
   PagedAttnArgs a{};
@@ -468,12 +478,13 @@ extern "C" int sarathi_paged_attention(
   a.num_indices = num_pages > 0 ? (int32_t)num_kv_indices : 0;  // no page: no key
   a.causal = causal != 0;
   a.window = window_left < 0 ? -1 : window_left < 0x3fffffff ? (int32_t)window_left : 0x3fffffff;
+  a.fill = fill;
   a.scale_log2 = sm_scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   const bool vec = head_size % 8 == 0 && aligned16(query) && aligned16(k_cache) &&
                    aligned16(v_cache) && aligned16(out) && query_stride % 8 == 0 &&
                    out_stride % 4 == 0 && page_stride % 8 == 0 && entry_stride % 8 == 0;
-  if (!vec) {
+  if (!vec || num_seqs == 0) {
     const dim3 grid((unsigned)num_tokens, (unsigned)num_heads);
     if (dtype == kBF16)
       hipLaunchKernelGGL((paged_attn_plain_kernel<kBF16>), grid, dim3(64), 0, st, a);
@@ -499,7 +510,9 @@ extern "C" int sarathi_paged_attention(
   } else {
     a.few.target = a.tile.target = 0;
   }
-  const int64_t groups = (cut ? p.items : p.uncut_items) * num_kv_heads;
+  int64_t groups = (cut ? p.items : p.uncut_items) * num_kv_heads;
+  a.item_groups = (uint32_t)groups;
+  if (fill) groups += num_tokens < kFillGroups ? num_tokens : kFillGroups;
   if (groups > 0x7fffffffLL) return SARATHI_ERR_UNSUPPORTED;
   // offsets inside a share of sixteen keys are 32-bit
   const bool page16 = page_size % 16 == 0 && a.entry_stride < (1 << 26);
@@ -510,4 +523,19 @@ extern "C" int sarathi_paged_attention(
   const int rc = launch_paged_attn(a, dtype, page16, groups, st);
   if (rc != SARATHI_OK || !cut) return rc;
   return dtype == kBF16 ? launch_join<kBF16>(a, st) : launch_join<kF16>(a, st);
+}
+
+extern "C" int sarathi_paged_attention(
+    const void* query, const void* k_cache, const void* v_cache, void* out, float* lse,
+    const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+    const int32_t* kv_last_page_len, int64_t num_tokens, int64_t num_seqs, int64_t num_kv_indices,
+    int64_t num_pages, int num_heads, int num_kv_heads, int head_size, int page_size,
+    int64_t query_stride, int64_t out_stride, int64_t page_stride, int64_t entry_stride,
+    float sm_scale, int causal, int64_t window_left, int64_t max_query_len, void* workspace,
+    int64_t workspace_bytes, int dtype, void* stream) {
+  return sarathi_paged_attention_fill(query, k_cache, v_cache, out, lse, qo_indptr, kv_indptr, kv_indices,
+                                      kv_last_page_len, num_tokens, num_seqs, num_kv_indices, num_pages,
+                                      num_heads, num_kv_heads, head_size, page_size, query_stride, out_stride,
+                                      page_stride, entry_stride, sm_scale, causal, window_left, max_query_len,
+                                      workspace, workspace_bytes, dtype, 0, stream);
 }

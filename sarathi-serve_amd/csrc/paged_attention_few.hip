@@ -12,7 +12,7 @@ __global__ __launch_bounds__(64 * kAttnWaves) void paged_attn_few_kernel(PagedAt
   extern __shared__ u32x4 few_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
   const AttnItem it = attn_item(a, blockIdx.x / (uint32_t)a.kv_heads, blockIdx.x == 0);
-  if (it.r < 0) return;
+  if (it.r < 0) return attn_fill(a);
   few_item<DT, DP, RT, PAD, PAGE16>(a, it, h, (lds_char*)few_lds);
 }
 

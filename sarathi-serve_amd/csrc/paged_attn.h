@@ -58,6 +58,8 @@ struct PagedAttnArgs {
   int32_t seqs, tokens, heads, kv_heads, group, head_size;
   int32_t page_size, num_pages, num_indices;
   int32_t causal, window;                 // window < 0: none
+  int32_t fill;           // rows of no request: 1: lse becomes -inf, 2: out becomes 0, 3: both
+  uint32_t item_groups;   // workgroups of the items; those behind them fill
   float scale_log2;                       // softmax scale * log2(e)
   AttnClass few, tile;                    // requests of up to few.max_rows rows; those of more
 };
@@ -103,6 +105,23 @@ SK_DEV int64_t attn_entry(const PagedAttnArgs& a, const AttnSeq& x, int32_t pos)
   const int32_t pg = attn_page_of(a, pos);
   const int32_t page = attn_clip_page(a, a.kv_indices[x.kv0 + pg]);
   return page * a.page_stride + (int64_t)(pos - pg * a.page_size) * a.entry_stride;
+}
+
+// Rows in front of the first request and behind the last one.  A few workgroups of 256 threads behind
+// those of the items, which find none, fill them; rows are 8-byte aligned here.  (Filled by the items'
+// own workgroups they cost the chunks' loop 1 %; told apart before the search, short decodes 5 %.)
+SK_DEV void attn_fill(const PagedAttnArgs& a) {
+  if (blockIdx.x < a.item_groups) return;
+  const int32_t lo = clamp_i32(a.qo_indptr[0], 0, a.tokens), hi = clamp_i32(a.qo_indptr[a.seqs], lo, a.tokens);
+  const int32_t rows = lo + a.tokens - hi;
+  for (int64_t i = blockIdx.x - a.item_groups; i < rows; i += gridDim.x - a.item_groups) {
+    const int64_t tok = i < lo ? i : hi + (i - lo);
+    if (a.fill & 2)
+      for (int32_t d = threadIdx.x * 4; d < a.heads * a.head_size; d += 64 * kAttnWaves * 4)
+        *reinterpret_cast<u32x2*>(reinterpret_cast<char*>(a.out) + (tok * a.out_stride + d) * 2) = u32x2{0, 0};
+    if (a.fill & 1)
+      for (int32_t h = threadIdx.x; h < a.heads; h += 64 * kAttnWaves) a.lse[tok * a.heads + h] = -INFINITY;
+  }
 }
 
 // ---- work items ------------------------------------------------------------------------------

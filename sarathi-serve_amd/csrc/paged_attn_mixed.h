@@ -17,7 +17,7 @@ void paged_attn_mixed_kernel(PagedAttnArgs a) {
   extern __shared__ u32x4 mixed_lds[];
   const uint32_t h = blockIdx.x % (uint32_t)a.kv_heads;
   const AttnItem it = attn_item(a, blockIdx.x / (uint32_t)a.kv_heads, blockIdx.x == 0);
-  if (it.r < 0) return;
+  if (it.r < 0) return attn_fill(a);
   if (it.tiled) tile_item<DT, DP, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
   else few_item<DT, DP, RT, PAD, PAGE16>(a, it, h, (lds_char*)mixed_lds);
 }

@@ -466,6 +466,7 @@ std::vector<torch::Tensor> build_paged_kv_metadata(
 
 // Attention of the batch's new tokens over the paged cache, a (K, V) pair or (v_cache empty) the
 // joint [num_pages, 2, page_size, heads, head_size] tensor.  Returns out, and lse where asked for.
+// Rows of no request: new tensors hold 0 and -inf there, a tensor that the caller gave is left as it was.
 // The scratch for cut contexts comes from torch's caching allocator on the launch stream, so calls
 // never share it.
 std::vector<torch::Tensor> paged_attention(
@@ -544,14 +545,14 @@ std::vector<torch::Tensor> paged_attention(
       (int)g.page_size, max_query_len);
   torch::Tensor workspace;
   if (ws > 0) workspace = torch::empty({ws}, query.options().dtype(torch::kUInt8));
-  raise_on(sarathi_paged_attention(
+  raise_on(sarathi_paged_attention_fill(
                query.data_ptr(), k_ptr, v_ptr, out.data_ptr(), lse, qo_indptr.data_ptr<int32_t>(),
                kv_indptr.data_ptr<int32_t>(), kv_indices.data_ptr<int32_t>(),
                kv_last_page_len.data_ptr<int32_t>(), tokens, seqs, kv_indices.numel(), cache.size(0),
                (int)heads, (int)g.heads, (int)g.head_size, (int)g.page_size, tokens > 1 ? qs : width,
                tokens > 1 ? os : width, g.page_stride, g.entry_stride, (float)scale, causal ? 1 : 0,
                window_left, max_query_len, ws > 0 ? workspace.data_ptr() : nullptr, ws,
-               dtype_code(query, op), scope.stream),
+               dtype_code(query, op), out_or_none.has_value() ? 1 : 3, scope.stream),
            op);
   return result;
 }

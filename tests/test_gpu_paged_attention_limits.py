@@ -170,3 +170,98 @@ def test_inputs_that_require_a_gradient_are_refused(ops, dev):
             merge(*args)
         with torch.no_grad():
             assert torch.equal(merge(*args)[0], want)
+
+
+# ---- rows of no request -------------------------------------------------------------------------------
+
+def dirty(dev, *shapes):
+    """Leaves NaN in the memory that the next tensors of these shapes are made of."""
+    held = [torch.full(s, float("nan"), dtype=t, device=dev) for s, t in shapes]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("front,behind", [(0, 5), (3, 0), (2, 300)])
+@pytest.mark.parametrize("new,total,heads,kv_heads,head_size,hint", [
+    ([1] * 5, [40, 3000, 1, 77, 300], 8, 2, 128, 1),                    # few rows, a cut context
+    ([70, 1, 9], [70, 500, 2000], 8, 1, 64, 0),                         # chunks beside single tokens
+    ([40, 2], [40, 90], 4, 2, 256, 0),
+    ([3, 1], [30, 9], 5, 1, 20, 0),                                     # the plain kernel
+    ([1] * 600, [1 + i % 40 for i in range(600)], 4, 2, 64, 1),         # planned
+    ([0, 0], [9, 0], 4, 2, 64, 0),                                      # requests without a new token
+])
+def test_rows_of_no_request_are_defined(ops, dev, front, behind, new, total, heads, kv_heads, head_size, hint):
+    """New outputs hold 0 and -inf in front of and behind the requests, whatever the queries there hold;
+    an output that was passed in is left alone there, and the new lse beside it is -inf."""
+    b = build_batch(52, 16, new, total, heads, kv_heads, head_size, torch.bfloat16)
+    d = to_dev(b, dev)
+    n = sum(new)
+    T = front + n + behind
+    q = torch.full((T, heads, head_size), float("nan"), dtype=torch.bfloat16, device=dev)
+    q[front:front + n] = d["query"]
+    index = (d["qo_indptr"] + front, d["kv_indptr"], d["kv_indices"], d["last"])
+    f, want = ops.kv_cache_ops.paged_attention, reference(b)
+    outside = torch.ones(T, dtype=torch.bool, device=dev)
+    outside[front:front + n] = False
+    for flat in (False, True):
+        dirty(dev, (q.shape, q.dtype), (q.shape[:2], torch.float32))
+        out, lse = f(q.flatten(1) if flat else q, d["cache"], *index, max_query_len=hint, return_lse=True)
+        assert bool((out[outside] == 0).all()) and bool((lse[outside] == -torch.inf).all())
+        check(b, out[front:front + n], lse[front:front + n], want)
+        dirty(dev, (q.shape, q.dtype))
+        only = f(q, d["cache"], *index, max_query_len=hint)
+        assert torch.equal(only.view_as(out), out)
+    given = torch.full((T, heads + 1, head_size), 3.0, dtype=torch.bfloat16, device=dev)
+    dirty(dev, (q.shape[:2], torch.float32))
+    res, lse2 = f(q, d["cache"], *index, max_query_len=hint, return_lse=True, out=given[:, :heads])
+    assert bool((given[outside] == 3).all()) and bool((given[:, heads] == 3).all())
+    assert torch.equal(res[~outside], out.view_as(q)[~outside]) and torch.equal(lse2, lse)
+
+
+def test_rows_without_any_request(ops, dev):
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    zero = torch.zeros(1, dtype=torch.int32, device=dev)
+    cache = torch.zeros((2, 2, 16, 2, 64), dtype=torch.float16, device=dev)
+    q = torch.full((37, 6, 64), float("nan"), dtype=torch.float16, device=dev)
+    dirty(dev, (q.shape, q.dtype), (q.shape[:2], torch.float32))
+    out, lse = ops.kv_cache_ops.paged_attention(q, cache, zero, zero, none, none, return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -torch.inf).all())
+    given = torch.full_like(q, 3.0)
+    ops.kv_cache_ops.paged_attention(q, cache, zero, zero, none, none, out=given)
+    assert bool((given == 3).all())
+
+
+def test_a_captured_padded_step_returns_defined_rows(ops, dev):
+    """Metadata and attention into new outputs, captured once: at every replay the rows behind the batch are
+    0 and -inf, whatever the replay before left in them."""
+    import sarathi_amd.layers as layers
+    heads, kv_heads, D, page, R, M = 8, 2, 64, 16, 6, 40
+    g = gen(53)
+    cache = randn((R * M, 2, page, kv_heads, D), g).to(dev)
+    tables = torch.randperm(R * M, generator=g).to(torch.int32).reshape(R, M).to(dev)
+    query_lens, seq_lens = (torch.zeros(R, dtype=torch.int32, device=dev) for _ in range(2))
+    q = torch.full((R, heads, D), float("nan"), dtype=torch.bfloat16, device=dev)
+
+    def step():
+        meta = layers.build_append_metadata_on_device(query_lens, seq_lens, tables, page, R, max_query_len=1)
+        return meta.attention(q, cache, return_lse=True)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out, lse = step()
+    for lens in ([600, 1, 16, 17, 300, 64], [5, 400], [], [640, 2, 1]):
+        n = len(lens)
+        query_lens.copy_(torch.tensor([1] * n + [0] * (R - n), dtype=torch.int32))
+        seq_lens.copy_(torch.tensor(lens + [0] * (R - n), dtype=torch.int32))
+        q[:n] = randn((n, heads, D), g).to(dev)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, z = out.clone(), lse.clone()
+        assert bool((got[n:] == 0).all()) and bool((z[n:] == -torch.inf).all())
+        assert bool(got[:n].isfinite().all()) and bool(z[:n].isfinite().all())
+        eager, eager_z = step()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, got) and torch.equal(eager_z, z)

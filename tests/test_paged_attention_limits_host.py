@@ -30,3 +30,17 @@ def test_workspace_does_not_grow_with_requests_that_are_not_cut(workspace, h, hk
     for R in (1, 16, 300, 600, 4096, 8192, 65536):
         size = workspace(R, R, 64 * R, h, hk, d, 16, hint)
         assert 0 < size <= states + 16 * R + 8192, (R, size)
+
+
+def test_fill_of_rows_of_no_request():
+    import sarathi_amd  # noqa: F401
+    f = ctypes.CDLL(LIB).sarathi_paged_attention_fill
+    vp, cf = ctypes.c_void_p, ctypes.c_float
+    p = ctypes.cast(ctypes.create_string_buffer(4096), vp)
+
+    def call(fill, T=1, R=1, out=p, lse=None):
+        return f(p, p, p, out, vp(lse), p, p, p, p, i64(T), i64(R), i64(1), i64(1), ci(4), ci(2), ci(16), ci(16), i64(64),
+                 i64(64), i64(1024), i64(32), cf(1.0), ci(1), i64(-1), i64(0), vp(None), i64(0), ci(2), ci(fill), vp(None))
+    assert call(-1) == -1 and call(4) == -1
+    assert call(3, T=0) == 0 and call(0, R=0) == 0 and call(1, R=0) == 0      # no lse: nothing to fill
+    assert call(2, R=0, out=vp(None)) == -1
