@@ -306,7 +306,10 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   const int group = heads / kv_heads;
   const int64_t longest = max_query_len > 0 && max_query_len < tokens ? max_query_len : tokens;
   const int64_t most_rows = longest * group, all_rows = tokens * group;
-  const int64_t capacity = indices * page_size;  // no sequence has more keys
+  // All sequences together have no more keys.  Beyond 2^36 a smaller number only makes parts longer, and
+  // the products below stay within 64 bits.
+  int64_t capacity = indices * page_size;
+  if (capacity > (int64_t)1 << 36) capacity = (int64_t)1 << 36;
   const int64_t units = compute_units();
   const int few_limit = head_size > 128 ? 32 : 64;
   int64_t few_tiles = 0, chunk_tiles = 0, few_target = 0, chunk_target = 0;

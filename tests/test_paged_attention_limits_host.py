@@ -44,3 +44,15 @@ def test_fill_of_rows_of_no_request():
     assert call(-1) == -1 and call(4) == -1
     assert call(3, T=0) == 0 and call(0, R=0) == 0 and call(1, R=0) == 0      # no lse: nothing to fill
     assert call(2, R=0, out=vp(None)) == -1
+
+
+@pytest.mark.parametrize("T,R,NI,page,h,hk,hint", [
+    (11620506, 11, 13441971, 339304936, 4, 1, 1), (38834252, 1, 10796720, 68632828, 8, 8, 1),
+    (23899935, 151737, 38281589, 8492708, 32, 8, 1), (1787488, 8505, 2522992, 1835743780, 8, 1, 1),
+    (2762704, 779143, 325257681, 148975915, 1, 1, 0), (1, 1, (1 << 31) - 2, (1 << 31) - 1, 8, 1, 1),
+    (1 << 29, 1, (1 << 31) - 2, (1 << 31) - 1, 1, 1, 0),
+])
+def test_workspace_of_the_largest_pages(workspace, T, R, NI, page, h, hk, hint):
+    """Sizes whose products pass 64 bits: the workspace stays the states of what fills the GPU a few times,
+    at most 4096 tiles of 64 rows and 1024 of 128, with 16 bytes a request."""
+    assert 0 < workspace(T, R, NI, h, hk, 128, page, hint) <= (4096 * 64 + 1024 * 128) * 130 * 4 + 16 * R + 8192
