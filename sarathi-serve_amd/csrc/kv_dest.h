@@ -78,14 +78,19 @@ SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
     const int64_t at = (int64_t)page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
     return k.a < 0 ? -1 : at;  // a select: no branch
   }
-  if ((k.a | k.b) < 0) return -1;
-  const uint32_t pos = (uint32_t)k.b;
+  // Selects and no branches, so that the lookups of several tokens run side by side; where there is no
+  // page to look up, some word that exists is read instead.  A token without a destination looks at
+  // position 0 of no pages.
+  const bool named = (k.a | k.b) >= 0;
+  const int32_t b = named ? k.a : 0;
+  const uint32_t pos = (uint32_t)(named ? k.b : 0);
   const uint32_t pg = pos / (uint32_t)d.page_size;
   const uint32_t entry = pos - pg * (uint32_t)d.page_size;
-  const int64_t first = d.kv_indptr[k.a], past = d.kv_indptr[(int64_t)k.a + 1];
-  if (first + pg >= past) return -1;
-  const int64_t page = d.kv_indices[first + pg];
-  return page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
+  const int32_t first = d.kv_indptr[b], past = d.kv_indptr[(int64_t)b + (named ? 1 : 0)];
+  const bool inside = (int32_t)pg < past - first;  // 32 bits: scalar comparisons end there
+  const int64_t page = *(inside ? d.kv_indices + ((int64_t)first + pg) : d.kv_indptr);
+  const int64_t at = page * d.page_stride_bytes + (int64_t)entry * d.entry_stride_bytes;
+  return inside ? at : -1;
 }
 SK_DEV int64_t kv_entry_resolve(const KvDest& d, KvEntryKey k) {
   return d.slot_mapping != nullptr ? kv_entry_resolve<true>(d, k) : kv_entry_resolve<false>(d, k);

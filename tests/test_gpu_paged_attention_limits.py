@@ -85,6 +85,40 @@ def test_append_stays_within_the_pages_that_fit(ops, dev, room, fused):
         assert torch.equal(part, small)
 
 
+@pytest.mark.parametrize("page", [1, 3, 16])
+@pytest.mark.parametrize("fused", [False, True])
+def test_append_of_padding_alone_and_among_tokens(ops, dev, page, fused):
+    """Tokens without a request, a position or both, by the lookup, at the smallest page too (the page of
+    position -1 would be 2^32 - 1 there); a batch of no request at all."""
+    heads, D = 2, 64
+    f, g = ops.kv_cache_ops, gen(page)
+    cache = randn((20, 2, page, heads, D), g).to(dev)
+    table = cos_sin_cache(64, D, THETA_LLAMA3, torch.bfloat16).to(dev)
+    pages = [3, 7, 5, 11, 2, 0]
+    for b, pos, indptr in (([-1] * 5, [-1] * 5, [0]), ([0, -1, 0, 1, -1, 0, 1, 1], [2, 0, -1, 0, -1, 0, -1, 2], [0, 3, 6])):
+        n = len(b)
+        qkv = randn((n, 4 * heads * D), g).to(dev)
+        q, k, v = qkv.split([2 * heads * D, heads * D, heads * D], dim=-1)
+        rope = torch.tensor([max(p, 0) for p in pos], device=dev)
+        wq, wk = q.clone(), k.clone()
+        if fused:
+            ops.pos_encoding_ops.rotary_embedding(rope, wq, wk, D, table, True)
+        want = cache.clone()
+        for i, (r, x) in enumerate(zip(b, pos)):
+            if r >= 0 and x >= 0:
+                no = pages[indptr[r] + x // page]
+                want[no, 0, x % page], want[no, 1, x % page] = wk[i].view(heads, D), v[i].view(heads, D)
+        got = cache.clone()
+        index = (i32(dev, b), i32(dev, pos), got, i32(dev, pages), i32(dev, indptr))
+        if fused:
+            f.rotary_embedding_append_paged_kv(rope, q.clone(), k.clone(), v, D, table, True, *index)
+        else:
+            f.append_paged_kv_cache(k, v, *index)
+        assert torch.equal(got, want)
+        slots = f.get_kv_slot_mapping(*index[:2], *index[3:], page).tolist()
+        assert all((s < 0) == (r < 0 or x < 0) for s, r, x in zip(slots, b, pos))
+
+
 # ---- index vectors that are no batch's --------------------------------------------------------------
 
 def test_items_that_more_than_one_request_claims(ops, dev):
