@@ -313,7 +313,8 @@ static AttnPlan plan_attention(int64_t tokens, int64_t seqs, int64_t indices, in
   const int64_t units = compute_units();
   const int few_limit = head_size > 128 ? 32 : 64;
   int64_t few_tiles = 0, chunk_tiles = 0, few_target = 0, chunk_target = 0;
-  // two workgroups per compute unit; one where a chunk's tile has long heads
+  // Two workgroups per compute unit; one where a chunk's tile has long heads.  Few rows of heads above
+  // 128 fit once as well, but count as two: their parts are half as long as filling the GPU once asks for.
   const int64_t room = 2 * units, tile_room = head_size > 128 ? units : room;
   p.few.fill = room / kv_heads > 0 ? (int32_t)(room / kv_heads) : 1;
   p.tile.fill = tile_room / kv_heads > 0 ? (int32_t)(tile_room / kv_heads) : 1;

@@ -1,6 +1,6 @@
 // The attention kernel of batches without chunks: every work item is a tile of few rows
 // (paged_attn_few.h).  Four waves and 66 KiB of LDS per workgroup, so that two share a compute unit
-// and one's start and end run beside the other's stream.
+// and one's start and end run beside the other's stream (heads above 128: 130 KiB, one to a unit).
 #include "launch.h"
 #include "paged_attn_few.h"
 #include "paged_attn_launch.h"

@@ -17,13 +17,14 @@
 // Chunks of 16 bytes are stored swizzled so that operand reads meet no bank twice: K by XOR with the
 // row, V by XOR of its 64-byte pieces with the row.  Built with the products' results in vector
 // registers (build.py): as accumulators they cost a move per score.
-// Measured with one chunk of 4096 tokens at 12288, 32 + 8 heads of 128, bfloat16: 0.89 - 0.92 ms,
-// 1.05 PFLOP/s, where a library product of 8192^3 reaches 1.2; with zeros for data, which leave the
-// clock alone, it runs a quarter faster.  Eight waves sharing their keys (one workgroup per compute
+// Measured with one chunk of 4096 tokens at 12288, 32 + 8 heads of 128, bfloat16: 0.89 - 0.95 ms by
+// machine, 1.01 - 1.08 PFLOP/s, where a library product of 8192^3 reaches 1.2, once the clock has settled
+// (the first launches after idling take up to 1.2 ms); with zeros for data, which leave the clock alone,
+// it runs a quarter faster.  Eight waves sharing their keys (one workgroup per compute
 // unit) were 2 % faster there, 3 % slower on four ragged chunks, 4 % on a hybrid batch and 25 % on 512
 // tokens at 8192; four waves of 64 rows (half the LDS reads, one wave per SIMD) took 1.08 ms; the
 // softmax spread evenly over both products, or a raised wave priority for the second, changed nothing.
-// Heads of 256, 64 + 8 of them, 4096 tokens at 4096: 1.64 ms, 1.01 PFLOP/s (4.72 ms in tiles of 32 rows).
+// Heads of 256, 64 + 8 of them, 4096 tokens at 4096: 1.64 - 1.67 ms, 0.99 - 1.01 PFLOP/s (4.72 ms in tiles of 32 rows).
 // A launch of few tiles is bound by the chain of a wave alone on its SIMD: 1.4 us per 64 keys and tile.
 #pragma once
 
