@@ -470,7 +470,8 @@ SK_DEV AttnItem attn_find_item(const PagedAttnArgs& a, uint32_t want, bool map) 
 
 // The same for batches of many requests, where looking at all of them in every workgroup would cost
 // more than a launch (2048 decodes of up to 300 keys, 32 + 8 heads of 128: 0.90 ms, 0.34 this way): the
-// planning kernel has left the part lengths, the numbers of items, for either class the items before every request, and the state rows.
+// planning kernel has left the part lengths, the numbers of items, for either class the items before
+// every request, and the state rows.
 SK_DEV AttnItem attn_planned_item(const PagedAttnArgs& a, uint32_t want) {
   const int lane = threadIdx.x & 63;
   AttnItem it = {};

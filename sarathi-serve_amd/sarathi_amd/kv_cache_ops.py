@@ -146,7 +146,8 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: PagedCache, qo_indptr: 
     Returns ``out`` (shaped like ``query``), with ``return_lse`` also the natural-log sums
     ``[num_tokens, num_heads]`` (float32) that ``merge_attention_states`` joins.  A token that sees no
     key gets 0 and -inf, and so do rows behind the last request, except that those of an ``out`` that
-    was passed in are left as they were.  ``out`` must not overlap ``query`` or the cache.  A value that a mask hides from some of a request's tokens only must be finite.
+    was passed in are left as they were.  ``out`` must not overlap ``query`` or the cache.  A value that
+    a mask hides from some of a request's tokens only must be finite.
     No gradients: inputs that require one are refused unless gradients are switched off."""
     if kv_layout != "NHD":
         raise ValueError("only the NHD page layout is supported, got %r" % (kv_layout,))
